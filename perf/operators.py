@@ -94,7 +94,8 @@ def draw(rng):
 
 
 def _int8_weight(n, k, g):
-    w = torch.randint(-90, 91, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    """Rows begin at multiples of 16 bytes, as a program lays its weights out when it loads them."""
+    w = torch.randint(-90, 91, (n, (k + 15) // 16 * 16), generator=g, device="cuda", dtype=torch.int8)[:, :k]
     return w, (0.5 + torch.rand(n, generator=g, device="cuda")) * (0.02 / 52.0)
 
 
