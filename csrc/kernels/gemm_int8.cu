@@ -1,0 +1,578 @@
+// Products in 8-bit integers:  y[t, n] = s[t] c[n] sum_k q[t, k] w[n, k]  (+ bias)(+ residual) | silu(gate) up.
+//
+// q are rows of activations in 8 bits with a factor s each (int8_rows.cuh), w a weight with a factor c per channel.  The sums are whole
+// numbers in 32 bits, exact for K up to 131072 (128 * 127 * K < 2^31), so their order does not matter and a product may be cut along K
+// wherever it pays; one rounding to the type of the result follows the factors, the bias and the residual.
+//
+// What bounds it: few rows, the stream of w from HBM (half of bf16's); many, the tensor cores, kind::i8 at twice the rate of
+// kind::f16 for the same bytes of operands.
+//
+// W is the M side of tcgen05.mma -- 128 channels a tile, TW = 2: 128 gate and their 128 up channels, two accumulators -- and the rows are its N
+// side, padded to a multiple of 16 only, up to 256 (128 when gated).  So one kernel serves one row, whose stage of the ring is W almost
+// alone, and thousands, 128 x 256 to a tile.  Warp 0 issues the TMA loads, warp 1 the products, warps 2 - 5 the epilogue: sums leave
+// TMEM for shared memory 32 rows at a time and come back a row per warp, so that 128 channels of a row are stored together.
+//
+// Division of the work:
+//   * no more tiles than SMs: a cluster of up to 8 CTAs shares a tile, each takes a part of K; the parts are summed over distributed shared
+//     memory;
+//   * else: whole tiles, dealt to one CTA per SM in rounds, the epilogue of a tile under the products of the next (two accumulators).  The
+//     tiles left for the last round, which would leave most SMs idle, are cut along K into one range per SM; CTAs that share a tile leave
+//     their sums in a workspace, and whichever comes last adds them up.  Ranges come first, so that those sums pass under whole tiles.
+#include <algorithm>
+
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "gemm_rows.cuh"
+#include "int8_rows.cuh"
+#include "ogb_kernels.h"
+
+
+namespace ogb {
+
+int make_tmap_u8_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols);
+
+constexpr int kI8K = 128;                    // 128 bytes: a row of the 128-byte swizzle
+constexpr int kI8Threads = 192;
+constexpr int kI8MaxK = 131072;
+constexpr int kI8Group = 16;                 // tiles of W that go together against all rows
+constexpr int kI8Stage = 32 * 128 * 4;       // staging of 32 rows of an accumulator
+
+struct Int8Params {
+  void* out;
+  const float* factor;                       // s
+  const float* channel;                      // c
+  const float* bias;                         // or null
+  const void* residual;                      // or null
+  long long ldc, ldr;
+  int out_elem, vec;                         // vec: results and residuals in pieces of four
+  int M, N, mn;                              // mn: rows of a tile, a multiple of 16
+  int n_tiles, m_tiles, tiles, k_blocks, stages;
+  int splits;                                // CTAs (a cluster) per tile; 0: whole tiles and ranges
+  int cut;                                   // the first `cut` tiles are cut into ranges
+  int* status;
+  int* ws;                                   // [CTA][2][TW][4 quarters][rows / 4][32 channels][4 rows]
+  unsigned int* counters;                    // [CTA], zero when the kernel starts
+};
+
+OGB_DEVICE void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// kind::i8: signed 8-bit A and B, both K-major, 32-bit sums that wrap (they never get that far).
+__host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
+  return (2u << 4)                      // D format: s32
+         | (1u << 7) | (1u << 10)       // A, B format: signed
+         | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Tiles in groups of kI8Group tiles of W: within a group W goes fastest, so that the tiles under way at one time (about 148) share both operands
+// in L2.
+OGB_DEVICE void i8_tile(const Int8Params& p, int tile, int& nt, int& mt) {
+  const int g = tile / (kI8Group * p.m_tiles), first = g * kI8Group;
+  const int wide = min(kI8Group, p.n_tiles - first), t = tile - first * p.m_tiles;
+  nt = first + t % wide;
+  mt = t / wide;
+}
+
+// The parts of tiles that a CTA computes, in order: of its range the tile it shares with the CTA before it, the one it shares with the CTA
+// after it and the whole ones; then its whole tiles.
+struct Int8Segs {
+  long long it0, it1, first_end, last_begin, mid;
+  int k_blocks, state = 0, tile, tiles, stride;
+  OGB_DEVICE explicit Int8Segs(const Int8Params& p) : k_blocks(p.k_blocks), tiles(p.tiles) {
+    stride = gridDim.x;
+    if (p.splits > 0) {
+      const long long base = static_cast<long long>(blockIdx.x / p.splits) * k_blocks;
+      const int rank = blockIdx.x % p.splits;
+      it0 = base + k_blocks * rank / p.splits;
+      it1 = base + k_blocks * (rank + 1) / p.splits;
+      tile = tiles;
+    } else {
+      const long long total = static_cast<long long>(p.cut) * k_blocks;
+      it0 = GemmWork::range_begin(total, gridDim.x, blockIdx.x);
+      it1 = GemmWork::range_begin(total, gridDim.x, blockIdx.x + 1);
+      tile = p.cut + blockIdx.x;
+    }
+    first_end = it0 % k_blocks != 0 ? min(it1, (it0 / k_blocks + 1) * k_blocks) : it0;
+    last_begin = it1 % k_blocks != 0 ? max(first_end, it1 / k_blocks * k_blocks) : it1;
+    mid = first_end;
+  }
+  OGB_DEVICE bool next(int& t, int& kb0, int& kb1) {
+    long long a = 0, b = 0;
+    if (state == 0) { a = it0; b = first_end; state = 1; }
+    if (state == 1 && a >= b) { a = last_begin; b = it1; state = 2; }
+    if (state == 2 && a >= b) {
+      if (mid < last_begin) {
+        a = mid;
+        b = mid = mid + k_blocks;
+      } else {
+        if (tile >= tiles) return false;
+        t = tile; kb0 = 0; kb1 = k_blocks;
+        tile += stride;
+        return true;
+      }
+    }
+    t = static_cast<int>(a / k_blocks);
+    kb0 = static_cast<int>(a - static_cast<long long>(t) * k_blocks);
+    kb1 = static_cast<int>(b - static_cast<long long>(t) * k_blocks);
+    return true;
+  }
+};
+struct Int8Cursor {
+  Int8Segs segs;
+  int tile = 0, kb = 0, kb1 = 0;
+  bool more;
+  OGB_DEVICE explicit Int8Cursor(const Int8Params& p) : segs(p) { more = segs.next(tile, kb, kb1); }
+  OGB_DEVICE void step() {
+    if (more && ++kb == kb1) more = segs.next(tile, kb, kb1);
+  }
+};
+
+// What a lane needs of its four neighbouring channels, for all rows of a tile.
+template <int TW>
+struct Int8Channels {
+  int n, n_out;                               // first column of the result, and how many there are
+  float c[TW][4], b[TW][4];
+  OGB_DEVICE Int8Channels(const Int8Params& p, int nt) {
+    const int lane = threadIdx.x & 31;
+    n = nt * 128 + 4 * lane;
+    n_out = p.N / TW;
+#pragma unroll
+    for (int w = 0; w < TW; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = min((nt * TW + w) * 128 + 4 * lane + i, p.N - 1);
+        c[w][i] = __ldg(p.channel + at);
+        b[w][i] = p.bias != nullptr ? __ldg(p.bias + at) : 0.f;
+      }
+  }
+};
+// Sums of row m (and of the up half) -> the stored result.
+template <int TW>
+OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m, float s, const int4& a, const int4& u) {
+  if (ch.n >= ch.n_out) return;
+  const int raw[4] = {a.x, a.y, a.z, a.w}, up[4] = {u.x, u.y, u.z, u.w};
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = fmaf(static_cast<float>(raw[i]) * s, ch.c[0][i], ch.b[0][i]);
+    if constexpr (TW == 2) {
+      const float w = fmaf(static_cast<float>(up[i]) * s, ch.c[TW - 1][i], ch.b[TW - 1][i]);
+      v[i] = __fdividef(v[i], 1.f + __expf(-v[i])) * w;
+    }
+  }
+  const size_t at = static_cast<size_t>(m) * p.ldc + ch.n, from = static_cast<size_t>(m) * p.ldr + ch.n;
+  if (p.vec != 0 && ch.n + 4 <= ch.n_out) {
+    if (p.out_elem == kElemF32) {
+      if (p.residual != nullptr) {
+        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + from);
+        v[0] += r.x; v[1] += r.y; v[2] += r.z; v[3] += r.w;
+      }
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+      return;
+    }
+    if (p.residual != nullptr) {
+      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + from);
+      const float2 lo = p.out_elem == kElemBf16 ? unpack_bf16(r.x) : __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+      const float2 hi = p.out_elem == kElemBf16 ? unpack_bf16(r.y) : __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+      v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = p.out_elem == kElemBf16 ? make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))
+                                                                                            : make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (ch.n + i < ch.n_out) store_elem(p.out, p.out_elem, at + i, p.residual != nullptr ? v[i] + load_elem(p.residual, p.out_elem, from + i) : v[i]);
+}
+
+// The epilogue warps, where whole tiles and ranges are computed.
+template <int TW>
+OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars, int* stage) {
+  const int q = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const long long total = static_cast<long long>(p.cut) * p.k_blocks;
+  const int slot = TW * 4 * acc_cols * 32;
+  volatile int* abort_flag = &bars->abort_flag;
+  volatile uint32_t* shared_last = &bars->shared_last;
+  pdl_wait();
+  const float* factor = after_wait(p.factor);
+  bool ok = true;
+  Int8Segs segs(p);
+  int tile, kb0, kb1;
+  for (int seg = 0; segs.next(tile, kb0, kb1); ++seg) {
+    const bool head = kb0 == 0, whole = head && kb1 == p.k_blocks;
+    const int buf = bufs == 2 ? (seg & 1) : 0;
+    const uint32_t buf_phase = (bufs == 2 ? seg >> 1 : seg) & 1;
+    int nt, mt;
+    i8_tile(p, tile, nt, mt);
+    const int rows = min(p.mn, p.M - mt * p.mn);
+    // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out the warps go on
+    // to arrive on the counters of their shared tiles.
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[buf], buf_phase))) {
+      ok = false;
+      if (lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *abort_flag = 1; }
+    }
+    tc_fence_after();
+    const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * TW * acc_cols;
+    int c_lo = 0, c_hi = 0;                                   // the CTAs that share the tile
+    if (!whole) {
+      c_lo = GemmWork::owner(total, gridDim.x, static_cast<long long>(tile) * p.k_blocks);
+      c_hi = GemmWork::owner(total, gridDim.x, static_cast<long long>(tile + 1) * p.k_blocks - 1) + 1;
+      if (ok) {
+        int4* dst = reinterpret_cast<int4*>(p.ws + static_cast<size_t>(blockIdx.x * 2 + (head ? 1 : 0)) * slot) + q * acc_cols * 8 + lane;
+#pragma unroll
+        for (int w = 0; w < TW; ++w) {
+#pragma unroll 1
+          for (int c = 0; c < rows; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32(t_addr + w * acc_cols + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (c + j < rows) __stcg(dst + (w * 4 * acc_cols + c + j) * 8, make_int4(r[j], r[j + 1], r[j + 2], r[j + 3]));
+          }
+        }
+      }
+      tc_fence_before();
+      __threadfence();
+      rows_epi_sync();
+      if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+      if (q == 0 && lane == 0) {
+        *shared_last = atomicAdd(p.counters + c_lo, 1u) == static_cast<unsigned int>(c_hi - c_lo - 1);
+        __threadfence();
+      }
+      rows_epi_sync();
+      const bool last = *shared_last != 0;
+      rows_epi_sync();
+      if (!__all_sync(0xffffffffu, ok && last)) continue;
+    } else if (!ok) {
+      continue;
+    }
+    const Int8Channels<TW> ch(p, nt);
+#pragma unroll 1
+    for (int c = 0; c < rows; c += 32) {
+#pragma unroll
+      for (int w = 0; w < TW; ++w) {
+        int v[32];
+        if (whole) {
+          uint32_t r[32];
+          tmem_ld_32x32(t_addr + w * acc_cols + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0;
+#pragma unroll 1
+          for (int x = c_lo; x < c_hi; ++x) {
+            // the first CTA of a tile holds its head (slot 1), the others a later part (slot 0)
+            const int4* src = reinterpret_cast<const int4*>(p.ws + static_cast<size_t>(x * 2 + (x == c_lo ? 1 : 0)) * slot) + ((w * 4 + q) * acc_cols + c) * 8 + lane;
+            int4 t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = __ldcg(src + j * 32);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { v[4 * j] += t[j].x; v[4 * j + 1] += t[j].y; v[4 * j + 2] += t[j].z; v[4 * j + 3] += t[j].w; }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) stage[(w * 32 + j) * 128 + q * 32 + lane] = v[j];
+      }
+      rows_epi_sync();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int m = q * 8 + j;
+        if (c + m < rows) {
+          const int row = mt * p.mn + c + m;
+          const int4 a = *reinterpret_cast<const int4*>(stage + m * 128 + 4 * lane);
+          const int4 u = *reinterpret_cast<const int4*>(stage + ((TW - 1) * 32 + m) * 128 + 4 * lane);
+          i8_store<TW>(p, ch, row, factor[row], a, u);
+        }
+      }
+      rows_epi_sync();
+    }
+    if (whole) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+    }
+  }
+}
+
+// All threads of a CTA, after their parts of the main loop: the epilogue of a tile that a cluster shares.  smem: the ring, free by then.
+template <int TW>
+OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int acc_cols, RowsBars* bars, uint8_t* smem, int ring_bytes) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* stage = reinterpret_cast<int*>(smem);
+  bool ok = true;
+  pdl_wait();
+  const float* factor = after_wait(p.factor);
+  const int tile = blockIdx.x / p.splits, rank = blockIdx.x % p.splits;
+  int nt, mt;
+  i8_tile(p, tile, nt, mt);
+  const int rows = min(p.mn, p.M - mt * p.mn);
+  const Int8Channels<TW> ch(p, nt);
+  if (warp >= 2) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[0], 0));      // every product has retired: the ring is free
+    if (!ok && lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1; }
+    tc_fence_after();
+  }
+  const int most = ring_bytes / (TW * 512) / 32 * 32;
+  for (int r0 = 0; r0 < rows; r0 += most) {
+    const int count = min(most, (rows - r0 + 31) / 32 * 32);
+    if (warp >= 2 && ok) rows_lay_out<TW>(tmem_base, acc_cols, r0, count, reinterpret_cast<float*>(stage));
+    if (p.splits > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+    for (int m = rank + p.splits * warp; m < count && r0 + m < rows; m += p.splits * warps) {
+      int4 s[TW];
+#pragma unroll
+      for (int w = 0; w < TW; ++w) {
+        int4 t[kRowsMaxSplit];
+        const int* src = stage + (static_cast<size_t>(w) * count + m) * 128 + 4 * lane;
+#pragma unroll
+        for (int x = 0; x < kRowsMaxSplit; ++x)
+          if (x < p.splits) t[x] = *reinterpret_cast<const int4*>(p.splits > 1 ? cooperative_groups::this_cluster().map_shared_rank(src, x) : src);
+        s[w] = t[0];
+#pragma unroll
+        for (int x = 1; x < kRowsMaxSplit; ++x)
+          if (x < p.splits) { s[w].x += t[x].x; s[w].y += t[x].y; s[w].z += t[x].z; s[w].w += t[x].w; }
+      }
+      const int row = mt * p.mn + r0 + m;
+      i8_store<TW>(p, ch, row, factor[row], s[0], s[TW - 1]);
+    }
+    // nobody overwrites or leaves what is being read
+    if (p.splits > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+  }
+}
+
+template <int TW>
+OGB_DEVICE bool i8_issue_mma(const Int8Params& p, uint8_t* smem, int stage_bytes, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars) {
+  const uint32_t idesc = make_idesc_i8(128, p.mn);
+  int stage = 0;
+  uint32_t phase = 0;
+  Int8Segs segs(p);
+  int tile, kb0, kb1;
+  for (int seg = 0; segs.next(tile, kb0, kb1); ++seg) {
+    const int buf = bufs == 2 ? (seg & 1) : 0;
+    const uint32_t buf_phase = (bufs == 2 ? seg >> 1 : seg) & 1;
+    if (!mbar_wait(&bars->tmem_empty[buf], buf_phase ^ 1)) return false;
+    tc_fence_after();
+    const uint32_t d_addr = tmem_base + buf * TW * acc_cols;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(&bars->full[stage], phase)) return false;
+      tc_fence_after();
+      const uint32_t sw = smem_u32(smem + stage * stage_bytes);
+      const uint64_t db = make_kmajor_sw128_desc(sw + TW * 128 * kI8K);
+#pragma unroll
+      for (int w = 0; w < TW; ++w) {
+        const uint64_t da = make_kmajor_sw128_desc(sw + w * 128 * kI8K);
+        // 32 values of K an instruction: +2 in the (>> 4) address field
+#pragma unroll
+        for (int k = 0; k < kI8K / 32; ++k) umma_i8(d_addr + w * acc_cols, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+      }
+      umma_commit(&bars->empty[stage]);
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    }
+    umma_commit(&bars->tmem_full[buf]);
+  }
+  return true;
+}
+
+template <int TW>
+__global__ void __launch_bounds__(kI8Threads, 1)
+gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q, const Int8Params p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int kStageW = TW * 128 * kI8K;
+  const int stage_bytes = kStageW + p.mn * kI8K;
+  const int ring_bytes = p.stages * stage_bytes;
+  RowsBars* bars = reinterpret_cast<RowsBars*>(smem + ring_bytes);
+  int* staging = reinterpret_cast<int*>(smem + ring_bytes + kRowsBarBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int acc_cols = (p.mn + 31) / 32 * 32;                  // the reads take 32 columns at a time
+  const int bufs = p.splits == 0 && 2 * TW * acc_cols <= 512 ? 2 : 1;
+  uint32_t tmem_cols = 32;
+  while (static_cast<int>(tmem_cols) < bufs * TW * acc_cols) tmem_cols *= 2;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_q);
+  }
+  const uint32_t tmem_base = rows_setup(bars, p.stages, 1, tmem_cols);
+  pdl_trigger();
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      auto load_w = [&](const Int8Cursor& c, int st) {
+        int nt, mt;
+        i8_tile(p, c.tile, nt, mt);
+        mbar_expect_tx(&bars->full[st], stage_bytes);
+#pragma unroll
+        for (int w = 0; w < TW; ++w)
+          tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (nt * TW + w) * 128);
+      };
+      // the first ring of W is on its way before the kernel ahead, which makes the rows, has ended
+      int ahead = 0;
+      for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
+      pdl_wait();
+      for (Int8Cursor c(p); c.more; c.step()) {
+        if (ahead > 0) {
+          --ahead;
+        } else {
+          if (!mbar_wait(&bars->empty[stage], phase ^ 1)) { ok = false; break; }
+          load_w(c, stage);
+        }
+        int nt, mt;
+        i8_tile(p, c.tile, nt, mt);
+        tma_load_2d(smem + stage * stage_bytes + kStageW, &tmap_q, &bars->full[stage], c.kb * kI8K, mt * p.mn);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) { atomicOr(p.status, kStatusWaitTimeout); *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1; }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer ------------------------------
+    if (lane == 0 && !i8_issue_mma<TW>(p, smem, stage_bytes, tmem_base, bufs, acc_cols, bars)) {
+      atomicOr(p.status, kStatusWaitTimeout);
+      *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1;
+    }
+    __syncwarp();
+  } else if (p.splits == 0) {
+    i8_epilogue<TW>(p, tmem_base, bufs, acc_cols, bars, staging);
+  }
+  if (p.splits > 0) i8_finish_cluster<TW>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
+  rows_teardown(bars, tmem_base, tmem_cols);
+}
+
+// ----------------------------------------------------------------------------------------
+// host side
+// ----------------------------------------------------------------------------------------
+// How a product is divided, from its sizes alone.
+struct Int8Plan {
+  int mn, m_tiles, n_tiles, tiles, k_blocks, cut;
+  bool clusters;
+  long long counter_bytes, ws_bytes;
+};
+static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
+  Int8Plan r{};
+  const int tw = gated ? 2 : 1, most = gated ? 128 : 256;
+  r.m_tiles = (M + most - 1) / most;
+  r.mn = ((M + r.m_tiles - 1) / r.m_tiles + 15) / 16 * 16;
+  r.m_tiles = (M + r.mn - 1) / r.mn;
+  r.n_tiles = (N + 128 * tw - 1) / (128 * tw);
+  r.tiles = r.m_tiles * r.n_tiles;
+  r.k_blocks = (K + kI8K - 1) / kI8K;
+  r.clusters = r.tiles <= sms;
+  if (!r.clusters) {
+    r.cut = r.tiles % sms;
+    if (r.cut > 0) {
+      r.counter_bytes = (static_cast<long long>(sms) * 4 + 1023) / 1024 * 1024;
+      r.ws_bytes = 2ll * sms * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
+    }
+  }
+  return r;
+}
+
+template <int TW>
+static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long long ldq, const void* w, long long ldw, int K, bool early, cudaStream_t stream) {
+  auto kernel = gemm_int8_kernel<TW>;
+  static OncePerDevice allowed;
+  int rc = allow_smem(allowed, kernel, kRowsSmemMax);
+  if (rc != 0) return rc;
+  const int stage_bytes = TW * 128 * kI8K + p.mn * kI8K;
+  const int extra = kRowsBarBytes + (plan.clusters ? 0 : TW * kI8Stage);
+  p.stages = std::min(kRowsMaxStages, (kRowsSmemMax - extra) / stage_bytes);
+  const int smem = p.stages * stage_bytes + extra;
+  int grid = ogb_num_sms();
+  if (plan.clusters) {
+    p.splits = rows_pick_splits(kernel, kI8Threads, smem, p.tiles, p.k_blocks);
+    grid = p.tiles * p.splits;
+  }
+  CUtensorMap mw, mq;
+  rc = make_tmap_u8_2d(&mw, w, p.N, K, ldw, 128, kI8K);
+  if (rc != 0) return rc;
+  rc = make_tmap_u8_2d(&mq, q, p.M, K, ldq, p.mn, kI8K);
+  if (rc != 0) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kI8Threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (p.splits > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = p.splits;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (early) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, mw, mq, p));
+}
+
+}  // namespace ogb
+
+using namespace ogb;
+
+// Bytes of workspace that a product needs: for its rows (when they come in a float type), its counters and the sums of shared tiles.
+static long long i8_rows_bytes(int M, int K) { return (static_cast<long long>(M) * ((K + 15) / 16 * 16) + 255) / 256 * 256; }
+static long long i8_factor_bytes(int M) { return (static_cast<long long>(M) * 4 + 255) / 256 * 256; }
+
+extern "C" int64_t ogb_gemm_int8_workspace(int M, int N, int K, int gated, int quantize) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Int8Plan plan = i8_plan(M, N, K, gated != 0, ogb_num_sms());
+  return plan.counter_bytes + plan.ws_bytes + (quantize != 0 ? i8_rows_bytes(M, K) + i8_factor_bytes(M) : 0);
+}
+
+extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void* q, const float* factor, int64_t ldq, const void* w, int64_t ldw,
+                             const float* channel, const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldc, int out_elem, int M, int N,
+                             int K, int gated, void* ws, int64_t ws_bytes, int* status, void* stream_) {
+  if (M < 0 || N < 0 || K < 1 || K > kI8MaxK || out_elem < 0 || out_elem >= kElemKinds) return -2;
+  if (M == 0 || N == 0) return 0;
+  if ((x == nullptr) == (q == nullptr) || (x != nullptr && (x_elem < 0 || x_elem >= kElemKinds)) || (q != nullptr && factor == nullptr)) return -5;
+  if ((ldw & 15) != 0 || ldw < K || (reinterpret_cast<uintptr_t>(w) & 15) != 0) return -4;
+  if (q != nullptr && ((ldq & 15) != 0 || ldq < K || (reinterpret_cast<uintptr_t>(q) & 15) != 0)) return -4;
+  if (gated != 0 && (N % 256) != 0) return -6;
+  const int sms = ogb_num_sms();
+  const Int8Plan plan = i8_plan(M, N, K, gated != 0, sms);
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const bool quantize = q == nullptr;
+  const long long rows_bytes = quantize ? i8_rows_bytes(M, K) : 0, factor_bytes = quantize ? i8_factor_bytes(M) : 0;
+  if (ws_bytes < rows_bytes + factor_bytes + plan.counter_bytes + plan.ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 255) != 0) return -8;
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  Int8Params p{};
+  p.counters = reinterpret_cast<unsigned int*>(at + rows_bytes + factor_bytes);
+  p.ws = reinterpret_cast<int*>(at + rows_bytes + factor_bytes + plan.counter_bytes);
+  const int counters = plan.counter_bytes > 0 ? sms : 0;
+  bool early = launch_overlap();
+  if (quantize) {
+    ldq = (K + 15) / 16 * 16;
+    float* f = reinterpret_cast<float*>(at + rows_bytes);
+    const int rc = launch_quantize_rows(x, reinterpret_cast<int8_t*>(at), f, M, K, ldx, ldq, x_elem, p.counters, counters, stream);
+    if (rc != 0) return rc;
+    q = at;
+    factor = f;
+    early = true;          // nothing but the kernel just launched is still running when this one starts: see pdl_wait
+  } else if (counters > 0) {
+    OGB_CUDA_CHECK(cudaMemsetAsync(p.counters, 0, static_cast<size_t>(counters) * 4, stream));
+    early = false;
+  }
+  p.out = out; p.factor = factor; p.channel = channel; p.bias = bias; p.residual = residual;
+  p.ldc = ldc; p.ldr = ldr; p.out_elem = out_elem;
+  const int piece = 4 * elem_bytes(out_elem);
+  p.vec = (reinterpret_cast<uintptr_t>(out) % piece == 0 && ldc % 4 == 0 &&
+           (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) % piece == 0 && ldr % 4 == 0))) ? 1 : 0;
+  p.M = M; p.N = N; p.mn = plan.mn; p.n_tiles = plan.n_tiles; p.m_tiles = plan.m_tiles; p.tiles = plan.tiles; p.k_blocks = plan.k_blocks;
+  p.cut = plan.cut; p.status = status;
+  return gated != 0 ? launch_int8<2>(plan, p, q, ldq, w, ldw, K, early, stream) : launch_int8<1>(plan, p, q, ldq, w, ldw, K, early, stream);
+}

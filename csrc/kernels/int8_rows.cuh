@@ -1,0 +1,121 @@
+// Rows of 8-bit integers with one factor each, the left side of the products of gemm_int8.cu.
+//
+//   factor = max |x| / 127,   q = round(127 x / max |x|), halves to even
+//
+// A row of zeros has factor 0; a row that holds an infinity or a NaN has factor NaN and zeros, so that whatever is multiplied by it is NaN.
+#pragma once
+#include "common.cuh"
+
+namespace ogb {
+
+enum Elem : int { kElemF32 = 0, kElemBf16 = 1, kElemF16 = 2 };
+constexpr int kElemKinds = 3;
+inline int elem_bytes(int elem) { return elem == kElemF32 ? 4 : 2; }
+// every row of a matrix begins at a multiple of 16 bytes
+inline int rows_aligned(const void* p, long long ld, int elem) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem_bytes(elem) & 15) == 0 ? 1 : 0;
+}
+
+OGB_DEVICE float load_elem(const void* p, int elem, size_t at) {
+  if (elem == kElemF32) return static_cast<const float*>(p)[at];
+  if (elem == kElemBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+  return __half2float(static_cast<const __half*>(p)[at]);
+}
+// Eight neighbouring values from column i on of a row that begins at value `row` and has n; zeros past its end.
+OGB_DEVICE void load8(const void* p, int elem, bool vec, size_t row, int i, int n, float (&f)[8]) {
+  if (vec && i + 8 <= n) {
+    if (elem == kElemF32) {
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + row + i);
+      const float4 a = s[0], b = s[1];
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+      return;
+    }
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + row + i);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = elem == kElemBf16 ? unpack_bf16(w[j]) : __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = i + j < n ? load_elem(p, elem, row + i + j) : 0.f;
+}
+OGB_DEVICE void store_elem(void* p, int elem, size_t at, float v) {
+  if (elem == kElemF32) static_cast<float*>(p)[at] = v;
+  else if (elem == kElemBf16) static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16(v);
+  else static_cast<__half*>(p)[at] = __float2half_rn(v);
+}
+OGB_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+OGB_DEVICE void store8(void* p, int elem, bool vec, size_t row, int i, int n, const float (&f)[8]) {
+  if (vec && i + 8 <= n) {
+    if (elem == kElemF32) {
+      float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + row + i);
+      d[0] = make_float4(f[0], f[1], f[2], f[3]);
+      d[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else if (elem == kElemBf16) {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + i) =
+          make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + i) =
+          make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (i + j < n) store_elem(p, elem, row + i + j, f[j]);
+}
+
+// What a row's values are multiplied by.  `peak` holds the bits of max |x|: as whole numbers they are ordered like the values, with
+// infinities and NaN above.
+struct RowCode {
+  float peak, inv, pre, factor;
+  bool bad;
+  OGB_DEVICE explicit RowCode(uint32_t peak_bits) {
+    bad = peak_bits >= 0x7f800000u;
+    peak = bad ? 0.f : __uint_as_float(peak_bits);
+    factor = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(peak, 127.f);
+    // Powers of two (exact) that keep 127 / peak and 127 x within the range of the type.
+    pre = peak > 0x1p100f ? 0x1p-40f : peak < 0x1p-90f ? 0x1p60f : 1.f;
+    inv = peak > 0.f ? __fdiv_rn(127.f, peak * pre) : 0.f;
+  }
+  // The product with the reciprocal is off by less than 2^-15 (three roundings of a value up to 127); only where it lies that near to a half
+  // does the quotient, in 64 bits, decide.
+  OGB_DEVICE int code(float x) const {
+    const float r = x * pre * inv;
+    float n = rintf(r);
+    if (fabsf(r - n) > 0.5f - 0x1p-14f) n = static_cast<float>(rint(static_cast<double>(x) * 127.0 / static_cast<double>(peak)));
+    return static_cast<int>(n);
+  }
+};
+OGB_DEVICE uint32_t pack_codes(int a, int b, int c, int d) {
+  return (static_cast<uint32_t>(a) & 255u) | (static_cast<uint32_t>(b) & 255u) << 8 | (static_cast<uint32_t>(c) & 255u) << 16 |
+         static_cast<uint32_t>(d) << 24;
+}
+// Eight codes from column i on; rows of q are a multiple of 16 bytes long, so that the last ones may pass the row's end.
+OGB_DEVICE void store_codes(int8_t* q, size_t row, int i, const RowCode& c, const float (&f)[8]) {
+  uint2 v = make_uint2(0, 0);
+  if (!c.bad && c.peak > 0.f) {
+    v.x = pack_codes(c.code(f[0]), c.code(f[1]), c.code(f[2]), c.code(f[3]));
+    v.y = pack_codes(c.code(f[4]), c.code(f[5]), c.code(f[6]), c.code(f[7]));
+  }
+  *reinterpret_cast<uint2*>(q + row + i) = v;
+}
+OGB_DEVICE uint32_t peak_bits8(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+  return m;
+}
+
+// Launches the kernel that turns rows of x into codes (int8_rows.cu).  counters: words it sets to zero for the kernel behind it.
+int launch_quantize_rows(const void* x, int8_t* q, float* factor, int rows, int cols, long long ldx, long long ldq, int elem, unsigned int* counters,
+                         int num_counters, cudaStream_t stream);
+
+}  // namespace ogb

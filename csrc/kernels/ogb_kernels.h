@@ -265,6 +265,25 @@ int ogb_argmax_f32(const float* logits, int* out_tokens, int rows, int vocab, in
 int ogb_sample_f32(const float* logits, int* out_tokens, const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                    const float* uniform, uint32_t* work, int rows, int vocab, int ld, void* stream);
 
+// Products in 8-bit integers (gemm_int8.cu, int8_rows.cu).  elem: 0 = fp32, 1 = bf16, 2 = fp16; rows of 8-bit values begin at multiples of 16 bytes.
+// quantize_rows: factor = max |x| / 127, q = round(127 x / max |x|) of every row.
+int ogb_quantize_rows(const void* x, void* q, float* factor, int rows, int cols, int64_t ldx, int64_t ldq, int elem, void* stream);
+// out = (q w^T) factor channel (+ bias)(+ residual), or silu(gate) up of it over blocks of 128 gate and 128 up rows of w (gated, N of them together).
+// Either x, float rows that the call quantises, or q and factor; ws: ogb_gemm_int8_workspace bytes for this call alone, 256-byte aligned.
+int64_t ogb_gemm_int8_workspace(int M, int N, int K, int gated, int quantize);
+int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void* q, const float* factor, int64_t ldq, const void* w, int64_t ldw,
+                  const float* channel, const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldc, int out_elem, int M, int N,
+                  int K, int gated, void* ws, int64_t ws_bytes, int* status, void* stream);
+// x_out = x_scale x + y_scale gate post(y), h = pre(x_out) (or q and factor of it); ldg 0: one gate for all rows.  Null: left out.
+int ogb_block_norm(const void* x, const void* y, const void* gate, const void* post, const void* pre, void* x_out, void* h, void* q,
+                   float* factor, int64_t ldx, int64_t ldy, int64_t ldg, int64_t ldxo, int64_t ldh, int64_t ldq, int rows, int cols,
+                   int x_elem, int y_elem, int gate_elem, int w_elem, int h_elem, int gate_sigmoid, float eps, float x_scale, float y_scale,
+                   void* stream);
+// Per row of logits: log probability of tokens[row] (a negative token asks for none: 0, rank -1), entropy (or null), rank (or null), the `top` likeliest (up
+// to 32) with theirs.
+int ogb_token_logprobs(const void* logits, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
+                       int rows, int vocab, int64_t ld, int top, int elem, int* status, void* stream);
+
 // MoE: softmax router with top-k (renormalised), device-side permutation by expert, grouped GEMM, combine.
 int ogb_moe_route_topk(const void* router_logits, int* topk_ids, float* topk_w, int tokens, int experts, int k,
                        int renormalize, int ld, void* stream);

@@ -13,6 +13,7 @@ import contextlib
 import math
 import os
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -532,6 +533,58 @@ def sample(logits, temperature, top_k, top_p, min_p, uniform, work=None, out=Non
     _native.check(rc, "ogb_sample")
     launch_counts["sample"] += 1
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` says about each row; None where it was not asked for."""
+    logprob: torch.Tensor                   # [rows] fp32
+    rank: torch.Tensor                      # [rows] int32: how many tokens are more likely
+    entropy: torch.Tensor | None            # [rows] fp32, in nats
+    top_ids: torch.Tensor | None            # [rows, top] int32, likeliest first, ties by index
+    top_logprobs: torch.Tensor | None       # [rows, top] fp32
+
+
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_TOP_LOGPROBS = 32
+
+
+@_timed("token_logprobs")
+def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
+    """Log probability of ``tokens[row]`` under the softmax of ``logits[row]`` (fp32, bf16 or fp16, any row stride), its rank, on request the
+    row's entropy and its ``top`` (at most 32) likeliest tokens.
+
+    A negative token asks for none: log probability 0 and rank -1.  A token past the vocabulary raises the status word's index bit, with NaN and
+    rank -1.  Logits of minus infinity weigh nothing; a row of nothing else, or with a NaN or plus infinity, has NaN for log probabilities and entropy (among the
+    likeliest, NaN comes last)."""
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or logits.shape[1] < 1:
+        raise ValueError(f"logits: a matrix of fp32, bf16 or fp16, not {tuple(logits.shape)} {logits.dtype}")
+    rows, vocab = logits.shape
+    if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):
+        raise ValueError(f"top = {top}: between 0 and {min(MAX_TOP_LOGPROBS, vocab)}")
+    if tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
+        raise ValueError(f"tokens: {rows} whole numbers (int32, int64) on the device of the logits")
+    if not logits.is_cuda:
+        return TokenLogprobs(*reference.token_logprobs(logits, tokens, top, entropy))
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if tokens.dtype != torch.int32:
+        tokens = tokens.clamp(-1, 2**31 - 1).int()         # what is past 32 bits stays past the vocabulary
+    tokens = tokens.contiguous()
+    dev = logits.device
+    # one allocation: log probability, rank, entropy, then the likeliest
+    words = torch.empty((3 + 2 * top) * rows, dtype=torch.float32, device=dev)
+    logprob, rank, ent = words[:rows], words[rows:2 * rows].view(torch.int32), words[2 * rows:3 * rows] if entropy else None
+    ids = lps = None
+    if top:
+        ids = words[3 * rows:(3 + top) * rows].view(torch.int32).view(rows, top)
+        lps = words[(3 + top) * rows:].view(rows, top)
+    guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+    with guard:
+        rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), _ptr(ent), rank.data_ptr(), _ptr(ids), _ptr(lps),
+                                               rows, vocab, logits.stride(0), top, _LOGIT_TYPES[logits.dtype], status_word(dev).data_ptr(), _stream())
+    _native.check(rc, "ogb_token_logprobs")
+    launch_counts["token_logprobs"] += 1
+    return TokenLogprobs(logprob, rank, ent, ids, lps)
 
 
 @_timed("spec_verify_greedy")

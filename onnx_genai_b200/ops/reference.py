@@ -274,6 +274,62 @@ def sample(logits, temperature, top_k, top_p, min_p, uniform):
     return out.to(logits.device)
 
 
+def token_logprobs(logits, tokens, top, entropy):
+    """-> (logprob, rank, entropy or None, top_ids or None, top_logprobs or None); see ops.token_logprobs."""
+    x = logits.double()
+    vocab = x.shape[1]
+    lp = torch.log_softmax(x, dim=1)
+    asked, known = tokens >= 0, (tokens >= 0) & (tokens < vocab)
+    at = torch.where(known, tokens.long(), 0)[:, None]
+    logprob = torch.where(known, lp.gather(1, at)[:, 0], torch.where(asked, math.nan, 0.0))
+    rank = torch.where(known, (x > x.gather(1, at)).sum(1), -1)
+    ent = torch.where(lp == -math.inf, 0.0, -lp.exp() * lp).sum(1).float() if entropy else None
+    if not top:
+        return logprob.float(), rank.int(), ent, None, None
+    nan = torch.isnan(x)
+    # NaN behind minus infinity: by value first, then, with everything else kept in order, whether it is a number
+    ids = torch.sort(torch.where(nan, -math.inf, x), dim=1, descending=True, stable=True).indices
+    ids = ids.gather(1, torch.sort(nan.gather(1, ids).int(), dim=1, stable=True).indices)[:, :top]
+    return logprob.float(), rank.int(), ent, ids.int(), lp.gather(1, ids).float()
+
+
+def quantize_rows(x):
+    """Rows in 8 bits -> (codes int8, factor fp32 a row).  Both quotients in 64 bits: the codes' decides on which side of a half it lies, and torch
+    divides CUDA tensors by a number through its reciprocal in 32."""
+    peak = x.float().abs().amax(1, keepdim=True)
+    bad = ~torch.isfinite(peak)
+    live = ~bad & (peak > 0)
+    q = torch.round(x.double() * 127.0 / torch.where(live, peak, 1.0).double())
+    return torch.where(live, q, 0.0).to(torch.int8), torch.where(bad, math.nan, (peak.double() / 127.0).float())[:, 0]
+
+
+def gemm_int8(a, w, w_scale, bias, residual, gated, out_dtype):
+    """Float rows, or (codes, factor), times an int8 weight with a factor per channel."""
+    q, s = a if isinstance(a, tuple) else quantize_rows(a)
+    y = (q.double() @ w.double().t()) * s.double()[:, None] * w_scale.double()
+    if bias is not None:
+        y = y + bias.double()
+    if gated:
+        y = y.view(y.shape[0], -1, 2, 128)
+        y = (torch.nn.functional.silu(y[:, :, 0]) * y[:, :, 1]).reshape(y.shape[0], -1)
+    if residual is not None:
+        y = y + residual.double()
+    return y.to(out_dtype)
+
+
+def block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid):
+    """-> (x' in fp32, h in fp32) of ops.int8.block_norm."""
+    new = x.float() * x_scale
+    if y is not None:
+        v = y.float()
+        if post is not None:
+            v = rms(v, post.float(), eps)
+        if gate is not None:
+            v = v * (torch.sigmoid(gate.float()) if gate_sigmoid else gate.float())
+        new = new + y_scale * v
+    return new, (rms(new, pre.float(), eps) if pre is not None else new)
+
+
 def spec_verify_greedy(logits, draft, k):
     """logits [S*(k+1), V]; draft [S, k] -> (accept_len [S], out_tokens [S, k+1] padded with -1)."""
     s = draft.shape[0]
