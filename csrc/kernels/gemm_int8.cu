@@ -122,13 +122,20 @@ struct Int8Segs {
     return true;
   }
 };
+// The k-blocks of a CTA one by one, with their tile's place.
 struct Int8Cursor {
+  const Int8Params& p;
   Int8Segs segs;
-  int tile = 0, kb = 0, kb1 = 0;
+  int nt = 0, mt = 0, kb = 0, kb1 = 0;
   bool more;
-  OGB_DEVICE explicit Int8Cursor(const Int8Params& p) : segs(p) { more = segs.next(tile, kb, kb1); }
+  OGB_DEVICE explicit Int8Cursor(const Int8Params& params) : p(params), segs(params) { part(); }
+  OGB_DEVICE void part() {
+    int tile;
+    more = segs.next(tile, kb, kb1);
+    if (more) i8_tile(p, tile, nt, mt);
+  }
   OGB_DEVICE void step() {
-    if (more && ++kb == kb1) more = segs.next(tile, kb, kb1);
+    if (++kb == kb1) part();
   }
 };
 
@@ -410,12 +417,10 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       auto load_w = [&](const Int8Cursor& c, int st) {
-        int nt, mt;
-        i8_tile(p, c.tile, nt, mt);
         mbar_expect_tx(&bars->full[st], stage_bytes);
 #pragma unroll
         for (int w = 0; w < TW; ++w)
-          tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (nt * TW + w) * 128);
+          tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (c.nt * TW + w) * 128);
       };
       // the first ring of W is on its way before the kernel ahead, which makes the rows, has ended
       int ahead = 0;
@@ -428,9 +433,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           if (!mbar_wait(&bars->empty[stage], phase ^ 1)) { ok = false; break; }
           load_w(c, stage);
         }
-        int nt, mt;
-        i8_tile(p, c.tile, nt, mt);
-        tma_load_2d(smem + stage * stage_bytes + kStageW, &tmap_q, &bars->full[stage], c.kb * kI8K, mt * p.mn);
+        tma_load_2d(smem + stage * stage_bytes + kStageW, &tmap_q, &bars->full[stage], c.kb * kI8K, c.mt * p.mn);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
       if (!ok) { atomicOr(p.status, kStatusWaitTimeout); *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1; }

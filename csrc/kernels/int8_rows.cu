@@ -56,7 +56,7 @@ struct QuantizeParams {
   int num_counters;
 };
 
-template <int V, bool WARP>
+template <int E, int V, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : kMostThreads) quantize_rows_kernel(const QuantizeParams p) {
   __shared__ uint32_t part[kMostThreads / 32];
   pdl_trigger();
@@ -69,28 +69,31 @@ __global__ void __launch_bounds__(WARP ? 128 : kMostThreads) quantize_rows_kerne
   const void* x = after_wait(p.x);
   const size_t at = static_cast<size_t>(row) * p.ldx;
   const int step = threads * 8;
-  float f[V][8];
+  Raw8<E> f[V];
   uint32_t peak = 0;
 #pragma unroll
-  for (int v = 0; v < V; ++v) load8(x, p.elem, p.vec != 0, at, tid * 8 + v * step, p.cols, f[v]);
+  for (int v = 0; v < V; ++v) f[v].load(x, p.vec != 0, at, tid * 8 + v * step, p.cols);
 #pragma unroll
-  for (int v = 0; v < V; ++v) peak = max(peak, peak_bits8(f[v]));
+  for (int v = 0; v < V; ++v) peak = f[v].peak(peak);
   // longer rows than the registers hold are read again below
   for (int i = tid * 8 + V * step; i < p.cols; i += step) {
-    float t[8];
-    load8(x, p.elem, p.vec != 0, at, i, p.cols, t);
-    peak = max(peak, peak_bits8(t));
+    Raw8<E> t;
+    t.load(x, p.vec != 0, at, i, p.cols);
+    peak = t.peak(peak);
   }
-  const RowCode code(row_max<WARP>(peak, part));
+  const RowCode code(row_max<WARP>(Raw8<E>::peak_float(peak), part));
   const size_t to = static_cast<size_t>(row) * p.ldq;
+  float t[8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = tid * 8 + v * step;
-    if (i < p.cols) store_codes(p.q, to, i, code, f[v]);
+    f[v].get(t);
+    if (i < p.cols) store_codes(p.q, to, i, code, t);
   }
   for (int i = tid * 8 + V * step; i < p.cols; i += step) {
-    float t[8];
-    load8(x, p.elem, p.vec != 0, at, i, p.cols, t);
+    Raw8<E> r;
+    r.load(x, p.vec != 0, at, i, p.cols);
+    r.get(t);
     store_codes(p.q, to, i, code, t);
   }
   if (tid == 0) p.factor[row] = code.factor;
@@ -105,21 +108,22 @@ static int row_threads(int rows, int cols) {
   return t;
 }
 
+template <int E>
+static int launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
+  const int t = row_threads(p.rows, p.cols), pieces = (p.cols + 7) / 8;
+  const dim3 grid(t == 32 ? (p.rows + 3) / 4 : p.rows), block(t == 32 ? 128 : t);
+  const bool one = pieces <= t, more = pieces > kVec * t;
+  auto kernel = t == 32 ? (one ? quantize_rows_kernel<E, 1, true> : quantize_rows_kernel<E, kVec, true>)
+                        : (one ? quantize_rows_kernel<E, 1, false> : more ? quantize_rows_kernel<E, 2 * kVec, false> : quantize_rows_kernel<E, kVec, false>);
+  return static_cast<int>(launch_overlapped(kernel, grid, block, 0, stream, p));
+}
+
 int launch_quantize_rows(const void* x, int8_t* q, float* factor, int rows, int cols, long long ldx, long long ldq, int elem, unsigned int* counters,
                          int num_counters, cudaStream_t stream) {
-  QuantizeParams p{x, q, factor, ldx, ldq, rows, cols, elem, rows_aligned(x, ldx, elem), counters, num_counters};
-  const int t = row_threads(rows, cols);
-  const int pieces = (cols + 7) / 8;
-  const bool one = pieces <= t;
-  cudaError_t e;
-  if (t == 32) {
-    const dim3 grid((rows + 3) / 4), block(128);
-    e = one ? launch_overlapped(quantize_rows_kernel<1, true>, grid, block, 0, stream, p) : launch_overlapped(quantize_rows_kernel<kVec, true>, grid, block, 0, stream, p);
-  } else {
-    const dim3 grid(rows), block(t);
-    e = one ? launch_overlapped(quantize_rows_kernel<1, false>, grid, block, 0, stream, p) : launch_overlapped(quantize_rows_kernel<kVec, false>, grid, block, 0, stream, p);
-  }
-  return static_cast<int>(e);
+  const QuantizeParams p{x, q, factor, ldx, ldq, rows, cols, elem, rows_aligned(x, ldx, elem), counters, num_counters};
+  if (elem == kElemF32) return launch_quantize<kElemF32>(p, stream);
+  if (elem == kElemBf16) return launch_quantize<kElemBf16>(p, stream);
+  return launch_quantize<kElemF16>(p, stream);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(WARP ? 128 : kMostThreads) block_norm_kernel(c
       if (gp != nullptr) {
         load8(gp, p.gate_elem, p.gate_vec != 0, static_cast<size_t>(row) * p.ldg, i, n, t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[v][j] *= p.gate_sigmoid != 0 ? 1.f / (1.f + expf(-t[j])) : t[j];
+        for (int j = 0; j < 8; ++j) y[v][j] *= p.gate_sigmoid != 0 ? __fdividef(1.f, 1.f + __expf(-t[j])) : t[j];
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[v][j] = fmaf(ry, y[v][j], p.x_scale * x[v][j]);

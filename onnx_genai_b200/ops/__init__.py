@@ -39,6 +39,15 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+# The stream's handle without the object around it, which takes 3 us to make; where torch has no such call, the public one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def current_index() -> int:
+    """Index of the current CUDA device (CUDA has to be up)."""
+    return torch.cuda.current_device()
+
+
 def status_word(device=None) -> torch.Tensor:
     """Per-device int32 word kernels OR error bits into (wait timeout, index out of range...)."""
     idx = torch.cuda.current_device() if device is None else torch.device(device).index or 0
@@ -569,19 +578,21 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
         logits = logits.contiguous()
     if tokens.dtype != torch.int32:
         tokens = tokens.clamp(-1, 2**31 - 1).int()         # what is past 32 bits stays past the vocabulary
-    tokens = tokens.contiguous()
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     dev = logits.device
-    # one allocation: log probability, rank, entropy, then the likeliest
-    words = torch.empty((3 + 2 * top) * rows, dtype=torch.float32, device=dev)
-    logprob, rank, ent = words[:rows], words[rows:2 * rows].view(torch.int32), words[2 * rows:3 * rows] if entropy else None
-    ids = lps = None
-    if top:
-        ids = words[3 * rows:(3 + top) * rows].view(torch.int32).view(rows, top)
-        lps = words[(3 + top) * rows:].view(rows, top)
-    guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
-    with guard:
-        rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), _ptr(ent), rank.data_ptr(), _ptr(ids), _ptr(lps),
-                                               rows, vocab, logits.stride(0), top, _LOGIT_TYPES[logits.dtype], status_word(dev).data_ptr(), _stream())
+    index = dev.index
+    if index != current_index():
+        with torch.cuda.device(index):
+            return token_logprobs(logits, tokens, top, entropy)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    rank = torch.empty(rows, dtype=torch.int32, device=dev)
+    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
+    ids = torch.empty(rows, top, dtype=torch.int32, device=dev) if top else None
+    lps = torch.empty(rows, top, dtype=torch.float32, device=dev) if top else None
+    rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ent.data_ptr() if entropy else 0, rank.data_ptr(),
+                                           ids.data_ptr() if top else 0, lps.data_ptr() if top else 0, rows, vocab, logits.stride(0), top,
+                                           _LOGIT_TYPES[logits.dtype], status_word(dev).data_ptr(), _raw_stream(index))
     _native.check(rc, "ogb_token_logprobs")
     launch_counts["token_logprobs"] += 1
     return TokenLogprobs(logprob, rank, ent, ids, lps)

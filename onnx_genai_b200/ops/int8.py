@@ -8,11 +8,12 @@ the statements of :mod:`onnx_genai_b200.ops.reference`.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
 
-from . import _native, _timed, launch_counts, reference, status_word
+from . import _native, _raw_stream, _timed, current_index, launch_counts, reference, status_word
 
 P, I, L, F = _native.P, _native.I, _native.L, _native.F
 _native.register("ogb_quantize_rows", [P] * 3 + [I] * 2 + [L] * 2 + [I, P])
@@ -35,53 +36,40 @@ class Int8Rows(NamedTuple):
         return self.q.float() * self.scale[:, None]
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _refuse(what):
+    raise ValueError(what)
 
 
-def _float_rows(t, name):
-    _need(t.dim() == 2 and t.dtype in ELEM, f"{name} must be a matrix of fp32, bf16 or fp16, not {tuple(t.shape)} {t.dtype}")
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _padded(rows, k, device, alloc=torch.empty):
-    return alloc(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
-
-
-class _on:
-    """Launches go to the tensors' device, whichever is current."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _padded(rows, k, device):
+    """[rows, k] int8 whose rows begin at multiples of 16 bytes."""
+    if k % 16 == 0:
+        return torch.empty(rows, k, dtype=torch.int8, device=device)
+    return torch.empty(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
 
 
 @_timed("quantize_rows")
 def quantize_rows(x) -> Int8Rows:
     """``scale = max |x| / 127`` and ``q = round(127 x / max |x|)`` (halves to even) of every row of ``x`` [rows, k] (fp32, bf16, fp16; any
-    row stride).  A row of zeros has scale 0; one that holds an infinity or a NaN has scale NaN and zeros."""
-    x = _float_rows(x, "x")
+    strides).  A row of zeros has scale 0; one that holds an infinity or a NaN has scale NaN and zeros."""
+    if x.dim() != 2 or x.dtype not in ELEM:
+        _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(x.shape)} {x.dtype}")
     rows, k = x.shape
-    _need(k > 0, "rows without values have no scale")
-    q = _padded(rows, k, x.device)
+    if k == 0:
+        _refuse("rows without values have no scale")
+    if k > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    dev = x.device
+    q = _padded(rows, k, dev)
     if not x.is_cuda:
         codes, scale = reference.quantize_rows(x)
         q.copy_(codes)
         return Int8Rows(q, scale)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _on(x.device) as stream:
-        rc = _native.load().ogb_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, k, x.stride(0), q.stride(0), ELEM[x.dtype], stream)
+    index = dev.index
+    if index != current_index():
+        with torch.cuda.device(index):
+            return quantize_rows(x)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    rc = _native.load().ogb_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, k, x.stride(0), q.stride(0), ELEM[x.dtype], _raw_stream(index))
     _native.check(rc, "ogb_quantize_rows")
     launch_counts["quantize_rows"] += 1
     return Int8Rows(q, scale)
@@ -89,14 +77,16 @@ def quantize_rows(x) -> Int8Rows:
 
 def quantize_weight(w) -> Int8Rows:
     """A weight [n, k] in 8 bits with a factor per output channel, laid out for :func:`gemm_int8`.  Weights have to be finite."""
-    _need(bool(torch.isfinite(w).all()), "a weight that is not finite cannot be held in 8 bits")
+    if not bool(torch.isfinite(w).all()):
+        _refuse("a weight that is not finite cannot be held in 8 bits")
     return quantize_rows(w)
 
 
 def quantize_gate_up(gate, up) -> Int8Rows:
     """Gate and up projections [inter, k] as one weight for ``epilogue="swiglu"``: blocks of 128 gate rows and their 128 up rows, ``inter``
     padded with zero rows to a multiple of 128 (the padded columns of the result are zero: pad the next weight's k with anything)."""
-    _need(gate.shape == up.shape and gate.dim() == 2, "gate and up projections have one shape")
+    if gate.shape != up.shape or gate.dim() != 2:
+        _refuse("gate and up projections have one shape")
     pad = (-gate.shape[0]) % 128
     if pad:
         zero = gate.new_zeros(pad, gate.shape[1])
@@ -113,55 +103,85 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.  ``residual`` has the type of the result; ``out`` may be the same tensor.  The result's
     type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else bf16.  Sums over K are exact; one rounding follows the
     factors, the bias and the residual."""
-    _need(epilogue in _EPI, f"epilogue {epilogue!r}: one of {', '.join(_EPI)}")
     rows = isinstance(a, Int8Rows)
     x = a.q if rows else a
     gated = epilogue == "swiglu"
-    _need(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], f"a {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
-    _need((x.dtype == torch.int8) if rows else x.dtype in ELEM, f"rows of {x.dtype}")
+    if epilogue not in _EPI:
+        _refuse(f"epilogue {epilogue!r}: one of {', '.join(_EPI)}")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        _refuse(f"a {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
     m, k = x.shape
-    n = w.shape[0]
-    _need(0 < k <= MAX_K, f"k = {k}: between 1 and {MAX_K}")
-    _need(w.dtype == torch.int8 and w.device == x.device, "w must be int8 on the device of a")
-    for t, name in ((w_scale, "w_scale"), (bias, "bias")):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous() and t.device == x.device),
-              f"{name}: {n} contiguous fp32 values on the device of a")
-    _need(w_scale is not None, "w_scale is needed")
-    _need(not gated or (n % 256 == 0 and residual is None), "swiglu takes a weight of quantize_gate_up and no residual")
-    _need(epilogue != "residual" or residual is not None, "the residual is missing")
+    n, dev = w.shape[0], x.device
+    if (x.dtype != torch.int8) if rows else (x.dtype not in ELEM):
+        _refuse(f"rows of {x.dtype}")
+    if not 0 < k <= MAX_K:
+        _refuse(f"k = {k}: between 1 and {MAX_K}")
+    if w.dtype != torch.int8 or w.device != dev:
+        _refuse("w must be int8 on the device of a")
+    if w_scale is None or not _channels(w_scale, n, dev) or not (bias is None or _channels(bias, n, dev)):
+        _refuse(f"w_scale and bias: {n} contiguous fp32 values each on the device of a")
+    if gated and (n % 256 or residual is not None):
+        _refuse("swiglu takes a weight of quantize_gate_up and no residual")
+    if epilogue == "residual" and residual is None:
+        _refuse("the residual is missing")
     n_out = n // 2 if gated else n
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16 if rows else x.dtype
-    _need(out_dtype in ELEM, f"results of {out_dtype}")
-    for t, name in ((out, "out"), (residual, "residual")):
-        _need(t is None or (t.shape == (m, n_out) and t.dtype == out_dtype and t.device == x.device and (n_out <= 1 or t.stride(1) == 1)),
-              f"{name}: [{m}, {n_out}] {out_dtype} with neighbouring columns on the device of a")
+    if out_dtype not in ELEM:
+        _refuse(f"results of {out_dtype}")
+    for t in (out, residual):
+        if t is not None and (t.shape != (m, n_out) or t.dtype != out_dtype or t.device != dev or (n_out > 1 and t.stride(1) != 1)):
+            _refuse(f"out and residual: [{m}, {n_out}] {out_dtype} with neighbouring columns on the device of a")
     if not x.is_cuda:
         y = reference.gemm_int8(a, w, w_scale, bias, residual, gated, out_dtype)
         return y if out is None else out.copy_(y)
-    _need(w.stride(1) == 1 and w.stride(0) % 16 == 0 and w.data_ptr() % 16 == 0, "rows of w must begin at multiples of 16 bytes: lay it out by quantize_weight")
+    ldw, c1 = w.stride()
+    ldx, x1 = x.stride()
+    if n == 1:                     # one row has no next: any stride will do
+        ldw = (k + 15) // 16 * 16
+    if m == 1:
+        ldx = (k + 15) // 16 * 16
+    if out is not None and m > 1 and out.stride(0) < n_out:
+        _refuse("rows of out overlap")
+    if (c1 != 1 and k > 1) or ldw % 16 or w.data_ptr() % 16 or ldw < k:
+        _refuse("rows of w must begin at multiples of 16 bytes: lay it out by quantize_weight")
     if rows:
-        _need(x.stride(1) == 1 and x.stride(0) % 16 == 0 and x.data_ptr() % 16 == 0, "8-bit rows must begin at multiples of 16 bytes")
-        _need(a.scale.dtype == torch.float32 and a.scale.shape == (m,) and a.scale.is_contiguous() and a.scale.device == x.device, "a.scale: a contiguous fp32 value a row")
-    elif k > 1 and x.stride(1) != 1:
+        if (x1 != 1 and k > 1) or ldx % 16 or x.data_ptr() % 16 or ldx < k:
+            _refuse("8-bit rows must begin at multiples of 16 bytes")
+        if not _channels(a.scale, m, dev):
+            _refuse("a.scale: a contiguous fp32 value a row on the device of a.q")
+    elif x1 != 1 and k > 1:
         x = x.contiguous()
+        ldx = k
+    index = dev.index
+    if index != current_index():
+        with torch.cuda.device(index):
+            return gemm_int8(a, w, w_scale, bias, residual, epilogue, out, out_dtype)
     if out is None:
-        out = torch.empty(m, n_out, dtype=out_dtype, device=x.device)
+        out = torch.empty(m, n_out, dtype=out_dtype, device=dev)
     if m == 0 or n == 0:
         return out
-    lib = _native.load()
-    with _on(x.device) as stream:
-        # the caller's own memory for as long as the call: the allocator hands it on in the stream's order, and a captured graph keeps its own
-        size = lib.ogb_gemm_int8_workspace(m, n, k, gated, not rows)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        rc = lib.ogb_gemm_int8(0 if rows else x.data_ptr(), 0 if rows else ELEM[x.dtype], x.stride(0), x.data_ptr() if rows else 0,
-                               a.scale.data_ptr() if rows else 0, x.stride(0) if rows else 0, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
-                               bias.data_ptr() if bias is not None else 0, residual.data_ptr() if residual is not None else 0,
-                               residual.stride(0) if residual is not None else 0, out.data_ptr(), out.stride(0), ELEM[out_dtype], m, n, k, gated,
-                               ws.data_ptr() if size else 0, size, status_word(x.device).data_ptr(), stream)
+    # the caller's own memory for as long as the call: the allocator hands it on in the stream's order, and a captured graph keeps its own
+    size = _workspace(m, n, k, gated, not rows)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    rc = _native.load().ogb_gemm_int8(0 if rows else x.data_ptr(), 0 if rows else ELEM[x.dtype], ldx, x.data_ptr() if rows else 0,
+                                      a.scale.data_ptr() if rows else 0, ldx, w.data_ptr(), ldw, w_scale.data_ptr(),
+                                      0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                                      0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0), ELEM[out_dtype], m, n, k, gated,
+                                      ws.data_ptr() if size else 0, size, status_word(dev).data_ptr(), _raw_stream(index))
     _native.check(rc, "ogb_gemm_int8")
     launch_counts["gemm_int8"] += 1
     return out
+
+
+def _channels(t, n, dev):
+    return t.dtype == torch.float32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == dev
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(m, n, k, gated, quantize):
+    """Bytes, from the sizes alone."""
+    return _native.load().ogb_gemm_int8_workspace(m, n, k, gated, quantize)
 
 
 @_timed("block_norm")
@@ -174,26 +194,39 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     type (None: no norm).  ``gate``: [hidden] or [rows, hidden], taken as it is or through a sigmoid.  ``h`` comes in ``out_dtype`` (that of ``out``, else of ``x``), or as
     :class:`Int8Rows` with ``int8=True``.  All of it is computed in 32 bits and rounded where it is stored; h is taken from x' before that is
     rounded.  ``hidden`` is at most 16384 on CUDA; the tensors' columns are neighbours."""
-    _need(x.dim() == 2 and x.dtype in ELEM, f"x must be a matrix of fp32, bf16 or fp16, not {tuple(x.shape)} {x.dtype}")
-    rows, n = x.shape
-    _need(n > 0, "rows without values")
-    dev = x.device
-    for t, name in ((y, "y"), (x_out, "x_out"), (out, "out"), (gate if gate is not None and gate.dim() == 2 else None, "gate")):
-        _need(t is None or (t.shape == x.shape and t.dtype in ELEM and t.device == dev and (n == 1 or t.stride(1) == 1)),
-              f"{name}: a matrix of x's shape and device with neighbouring columns")
-    _need(n == 1 or x.stride(1) == 1, "x: neighbouring columns")
-    vectors = [(post, "post"), (pre, "pre"), (gate if gate is not None and gate.dim() != 2 else None, "gate")]
-    for t, name in vectors:
-        _need(t is None or (t.shape == (n,) and t.dtype in ELEM and t.device == dev and t.is_contiguous()), f"{name}: {n} contiguous values on x's device")
-    _need(y is not None or (post is None and gate is None), "a post norm or a gate needs y")
-    _need(post is None or pre is None or post.dtype == pre.dtype, "post and pre weights have one type")
-    _need(x_out is None or x_out.dtype == x.dtype, "x_out has the type of x")
-    _need(not int8 or (out is None and out_dtype is None), "8-bit rows are made by the call")
+    if x.dim() != 2 or x.dtype not in ELEM:
+        _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(x.shape)} {x.dtype}")
+    shape, dev = x.shape, x.device
+    rows, n = shape
+    if n == 0:
+        _refuse("rows without values")
+    if x.stride(1) != 1 and n > 1:
+        _refuse("x: neighbouring columns")
+    wide = gate is not None and gate.dim() == 2
+    for t in (y, x_out, out, gate if wide else None):
+        if t is not None and (t.shape != shape or t.dtype not in ELEM or t.device != dev or (t.stride(1) != 1 and n > 1)):
+            _refuse("y, x_out, out and a gate for each token: matrices of x's shape and device with neighbouring columns")
+    for t in (post, pre, None if wide else gate):
+        if t is not None and (t.dim() != 1 or t.shape[0] != n or t.dtype not in ELEM or t.device != dev or not t.is_contiguous()):
+            _refuse(f"post, pre and a gate for each channel: {n} contiguous values on x's device")
+    if y is None and (post is not None or gate is not None):
+        _refuse("a post norm or a gate needs y")
+    if post is not None and pre is not None and post.dtype != pre.dtype:
+        _refuse("post and pre weights have one type")
+    if x_out is not None and x_out.dtype != x.dtype:
+        _refuse("x_out has the type of x")
+    for t in (x_out if x_out is not None else x, out):
+        if t is not None and rows > 1 and t.stride(0) < n:
+            _refuse("rows of x_out (or x, where it takes the new stream) and out do not overlap")
+    if int8:
+        if out is not None or out_dtype is not None:
+            _refuse("8-bit rows are made by the call")
+    else:
+        out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+        if out_dtype not in ELEM or (out is not None and out.dtype != out_dtype):
+            _refuse(f"results of {out_dtype}")
     if x_out is None and (y is not None or x_scale != 1.0):
         x_out = x
-    if not int8:
-        out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-        _need(out_dtype in ELEM and (out is None or out.dtype == out_dtype), f"results of {out_dtype}")
     if not x.is_cuda:
         new, h = reference.block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid)
         if int8:
@@ -206,19 +239,25 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
         if x_out is not None:
             x_out.copy_(new)
         return h
-    _need(n <= MAX_HIDDEN, f"hidden {n}: at most {MAX_HIDDEN}")
+    if n > MAX_HIDDEN:
+        _refuse(f"hidden {n}: at most {MAX_HIDDEN}")
+    index = dev.index
+    if index != current_index():
+        with torch.cuda.device(index):
+            return block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid, x_out, out, None if int8 else out_dtype, int8)
+    q = scale = None
     if int8:
         q, scale = _padded(rows, n, dev), torch.empty(rows, dtype=torch.float32, device=dev)
     elif out is None:
         out = torch.empty(rows, n, dtype=out_dtype, device=dev)
-    ptr = lambda t: 0 if t is None else t.data_ptr()                      # noqa: E731
-    ld = lambda t: 0 if t is None or t.dim() != 2 else t.stride(0)        # noqa: E731
-    kind = lambda t: 0 if t is None else ELEM[t.dtype]                    # noqa: E731
-    with _on(dev) as stream:
-        rc = _native.load().ogb_block_norm(
-            x.data_ptr(), ptr(y), ptr(gate), ptr(post), ptr(pre), ptr(x_out), ptr(out), q.data_ptr() if int8 else 0, scale.data_ptr() if int8 else 0,
-            x.stride(0), ld(y), ld(gate), ld(x_out), ld(out), q.stride(0) if int8 else 0, rows, n, ELEM[x.dtype], kind(y), kind(gate),
-            kind(post if post is not None else pre), kind(out), int(gate_sigmoid), eps, x_scale, y_scale, stream)
+    weight = post if post is not None else pre
+    rc = _native.load().ogb_block_norm(
+        x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if gate is None else gate.data_ptr(), 0 if post is None else post.data_ptr(),
+        0 if pre is None else pre.data_ptr(), 0 if x_out is None else x_out.data_ptr(), 0 if out is None else out.data_ptr(),
+        q.data_ptr() if int8 else 0, scale.data_ptr() if int8 else 0, x.stride(0), 0 if y is None else y.stride(0), gate.stride(0) if wide else 0,
+        0 if x_out is None else x_out.stride(0), 0 if out is None else out.stride(0), q.stride(0) if int8 else 0, rows, n, ELEM[x.dtype],
+        0 if y is None else ELEM[y.dtype], 0 if gate is None else ELEM[gate.dtype], 0 if weight is None else ELEM[weight.dtype],
+        0 if out is None else ELEM[out_dtype], gate_sigmoid, eps, x_scale, y_scale, _raw_stream(index))
     _native.check(rc, "ogb_block_norm")
     launch_counts["block_norm"] += 1
     return Int8Rows(q, scale) if int8 else out
