@@ -126,47 +126,91 @@ struct Raw8 {
   }
 };
 
+// Two 32-bit floats in one instruction.
+struct Float2 {
+  unsigned long long v;
+  OGB_DEVICE Float2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  OGB_DEVICE explicit Float2(float both) : Float2(both, both) {}
+  OGB_DEVICE explicit Float2(unsigned long long bits) : v(bits) {}
+  OGB_DEVICE float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+  OGB_DEVICE float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+};
+OGB_DEVICE Float2 operator*(Float2 a, Float2 b) { unsigned long long d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v)); return Float2(d); }
+OGB_DEVICE Float2 operator+(Float2 a, Float2 b) { unsigned long long d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v)); return Float2(d); }
+OGB_DEVICE Float2 fma2(Float2 a, Float2 b, Float2 c) { unsigned long long d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v)); return Float2(d); }
+
 // What a row's values are multiplied by.  `peak` holds the bits of max |x|: as whole numbers they are ordered like the values, with
 // infinities and NaN above.
 struct RowCode {
-  float peak, inv, factor;
-  bool bad;
+  float power;       // of two, keeps the row within the range of the type
+  float scale;       // 127 times that
+  float peak, inv;   // max |x| times that power, and its reciprocal
+  float factor;
+  bool none;         // zeros, or not a number
   OGB_DEVICE explicit RowCode(uint32_t peak_bits) {
-    bad = peak_bits >= 0x7f800000u;
-    peak = bad ? 0.f : __uint_as_float(peak_bits);
-    factor = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(peak, 127.f);
-    inv = peak > 0x1p-100f ? __fdiv_rn(127.f, peak) : 0.f;     // smaller ones: the quotient itself
+    const bool bad = peak_bits >= 0x7f800000u;
+    const float top = bad ? 0.f : __uint_as_float(peak_bits);
+    none = !(top > 0.f);
+    factor = bad ? __uint_as_float(0x7fc00000u) : __fdiv_rn(top, 127.f);
+    power = top > 0x1p60f ? 0x1p-40f : top < 0x1p-60f ? 0x1p70f : 1.f;
+    scale = 127.f * power;
+    peak = top * power;
+    inv = none ? 0.f : __frcp_rn(peak);
   }
-  // Eight codes.  The product with the reciprocal is off by less than 2^-15 (three roundings of a value up to 127); only where it lies that near
-  // to a half does the quotient, in 64 bits, decide.  Adding 3 * 2^22 rounds to a whole number, halves to even, and leaves it in the low byte of
-  // the sum: conversions run at an eighth of the rate of additions.
+  // Adding 3 * 2^22 rounds to a whole number, halves to even, and leaves it in the low byte of the sum (conversions run at an eighth of the rate
+  // of additions).
+  static constexpr float kMagic = 12582912.f;
+  OGB_DEVICE static uint2 bytes(const uint32_t (&u)[8]) {
+    return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+  }
+  // Eight codes of values of 11 bits or fewer (bf16, fp16).  127 x is exact; r, the product with the reciprocal, is within 2^-22 of the quotient, and
+  // r + inv (127 x - peak r), whose middle is exact, within a rounding: a quotient that is a half is found as one, and no other comes nearer
+  // to a half than 2^-20 of itself (127 x and half * peak are whole multiples of one unit with 19 bits).
+  OGB_DEVICE uint2 codes_short(const float (&f)[8]) const {
+    uint32_t u[8];
+    const Float2 s(scale), v(inv), m(-peak), magic(kMagic);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const Float2 x = Float2(f[j], f[j + 1]) * s, r = x * v;
+      const Float2 q = fma2(fma2(m, r, x), v, r) + magic;
+      u[j] = __float_as_uint(q.lo());
+      u[j + 1] = __float_as_uint(q.hi());
+    }
+    return none ? make_uint2(0, 0) : bytes(u);
+  }
+  // Eight codes of any values.  The product with 127 / max |x| is off by less than 2^-15; only where it lies that near to a half is the
+  // sign of 127 x - half * peak taken, exactly: both products are split into what they round to and the rest.
   OGB_DEVICE uint2 codes(const float (&f)[8]) const {
-    if (bad || !(peak > 0.f)) return make_uint2(0, 0);
-    constexpr float kMagic = 12582912.f, kNear = 0.5f - 0x1p-14f;
+    constexpr float kNear = 0.5f - 0x1p-14f;
     float s[8], far = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float r = f[j] * inv;
+      const float r = f[j] * scale * inv;
       s[j] = r + kMagic;
       far = fmaxf(far, fabsf(r - (s[j] - kMagic)));
     }
-    if (far > kNear || inv == 0.f) {
+    if (far > kNear) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float r = f[j] * inv;
-        if (inv == 0.f || fabsf(r - (s[j] - kMagic)) > kNear)
-          s[j] = static_cast<float>(rint(static_cast<double>(f[j]) * 127.0 / static_cast<double>(peak))) + kMagic;
+        const float x = f[j] * power, r = f[j] * scale * inv;
+        if (fabsf(r - (s[j] - kMagic)) > kNear) {
+          const float below = floorf(r), half = below + 0.5f;
+          const float a = x * 127.f, a_rest = fmaf(x, 127.f, -a), b = half * peak, b_rest = fmaf(half, peak, -b);
+          const float d = (a - b) + (a_rest - b_rest);       // a - b is exact, the two being that near
+          const float even = 2.f * rintf(0.5f * half);       // the even one of the two neighbours
+          s[j] = (d > 0.f ? below + 1.f : d < 0.f ? below : even) + kMagic;
+        }
       }
     }
     uint32_t u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(s[j]);
-    return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
-                      __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+    return none ? make_uint2(0, 0) : bytes(u);
   }
 };
 // Codes from column i on; rows of q are a multiple of 16 bytes long, so that the last ones may pass the row's end.
-OGB_DEVICE void store_codes(int8_t* q, size_t row, int i, const RowCode& c, const float (&f)[8]) { *reinterpret_cast<uint2*>(q + row + i) = c.codes(f); }
+OGB_DEVICE void store_codes(int8_t* q, size_t row, int i, uint2 codes) { *reinterpret_cast<uint2*>(q + row + i) = codes; }
 OGB_DEVICE uint32_t peak_bits8(const float (&f)[8]) {
   uint32_t m = 0;
 #pragma unroll

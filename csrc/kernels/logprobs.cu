@@ -3,15 +3,17 @@
 //   m = max x,  s = sum exp(x - m),  t = sum exp(x - m) (x - m)
 //   log p(i) = x_i - m - log s,   entropy = log s - t / s,   rank = |{j : x_j > x_token}|
 //
-// One pass over the row: every thread carries (m, s, t) of its values and rescales them when a new maximum turns up; the states of threads,
-// warps and CTAs join by the same rule.  What bounds it is the stream of logits from HBM (2 bytes a value), with exp(x - m) -- one a value,
-// 16 a clock and SM -- close behind.
+// One pass over the row: every thread carries (m, s, t) of its values, m being a value near their maximum, and rescales them when one turns up that
+// is 2 above it.  The states of threads, warps and CTAs join by the same rule.  What bounds it is the stream of logits from HBM (2 bytes
+// a value), with exp(x - m) -- one a value, 16 a clock and SM -- and the issue of instructions close behind: differences, products and sums
+// go two values at a time, maxima and comparisons of 16-bit logits too.
 //
-// The likeliest values are found in the same pass.  A value's key is its order as a whole number above its inverted index, so that no two are
-// equal and ties go to the lower index.  A CTA holds the best `top` keys so far; only a piece whose maximum reaches the last of them is looked
-// at.  Among the threads of a CTA with such a piece, the top-th best of their best keys bounds the row's top-th best from below, so
-// at most `top` threads hold anything above that bound: a round adds at most top * kPiece keys whatever the order of the values (a row that rises from
-// end to end costs rounds, never space).
+// The likeliest values come from the same pass.  A value's key is its order as a whole number above its inverted index, so that no two are equal and
+// ties go to the lower index.  Threads leave the maximum of every 32-byte piece of the row in shared memory; the top-th best of their own best is a bound
+// that at least `top` values reach, and then only pieces whose maximum reaches it are read again, about as many as `top`.  A row on which
+// many do (the largest values all in the columns of few threads) has its pieces taken in rounds, each of which keeps the best `top` and raises the
+// bound; among the threads of a round the bound of their best keys holds again, so it adds at most top * kPer keys: such rows cost
+// time, never space.
 //
 // A row is split over a cluster of CTAs where rows are few; the parts join over distributed shared memory.
 //
@@ -30,9 +32,11 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpBlocks = 2;               // 16-byte blocks a thread takes per round
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxSplit = 8;             // the portable cluster size
+constexpr int kLpSmem = 200 * 1024;        // maxima of a CTA's pieces, at most
+constexpr int kLpQuick = 64;               // pieces that are read again at once, at most
+constexpr float kLpSlack = 2.f;
 
 struct LogprobsParams {
   const void* logits;
@@ -68,38 +72,163 @@ OGB_DEVICE float lp_value(unsigned long long key) {
   return __uint_as_float((o & 0x80000000u) != 0 ? o & 0x7fffffffu : ~o);
 }
 
+OGB_DEVICE float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Logits of a type: 32 bytes of them in eight words.
 template <typename T>
 struct LpType;
-template <> struct LpType<float> { static constexpr int kPer = 4, kElem = kElemF32; };
-template <> struct LpType<__nv_bfloat16> { static constexpr int kPer = 8, kElem = kElemBf16; };
-template <> struct LpType<__half> { static constexpr int kPer = 8, kElem = kElemF16; };
+template <>
+struct LpType<float> {
+  static constexpr int kPer = 8, kElem = kElemF32;
+  using Max = float;                                       // as a piece's maximum is kept
+  OGB_DEVICE static float max_of(const uint32_t (&w)[8]) {
+    float m = __uint_as_float(w[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = fmaxf(m, __uint_as_float(w[j]));
+    return m;
+  }
+  template <typename F>
+  OGB_DEVICE static void pairs(const uint32_t (&w)[8], F&& f) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) f(Float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])));
+  }
+  OGB_DEVICE static int above(const uint32_t (&w)[8], float given) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n += __uint_as_float(w[j]) > given ? 1 : 0;
+    return n;
+  }
+  OGB_DEVICE static float value(const uint32_t (&w)[8], int j) { return __uint_as_float(w[j]); }
+  static constexpr uint32_t kNothing = 0xff800000u;        // a word of minus infinities
+};
+template <>
+struct LpType<__nv_bfloat16> {
+  static constexpr int kPer = 16, kElem = kElemBf16;
+  using Max = __nv_bfloat16;
+  OGB_DEVICE static __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+  OGB_DEVICE static float max_of(const uint32_t (&w)[8]) {
+    __nv_bfloat162 m = two(w[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = __hmax2(m, two(w[j]));
+    const __nv_bfloat16 one = __hmax(m.x, m.y);
+    return __bfloat162float(one);
+  }
+  template <typename F>
+  OGB_DEVICE static void pairs(const uint32_t (&w)[8], F&& f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f(Float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)));
+  }
+  OGB_DEVICE static int above(const uint32_t (&w)[8], float given) {
+    const __nv_bfloat162 g = __float2bfloat162_rn(given);
+    __nv_bfloat162 n = __hgt2(two(w[0]), g);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) n = __hadd2(n, __hgt2(two(w[j]), g));
+    const float2 f = __bfloat1622float2(n);
+    return static_cast<int>(f.x + f.y);
+  }
+  OGB_DEVICE static float value(const uint32_t (&w)[8], int j) { return __uint_as_float((j & 1) != 0 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
+  static constexpr uint32_t kNothing = 0xff80ff80u;
+};
+template <>
+struct LpType<__half> {
+  static constexpr int kPer = 16, kElem = kElemF16;
+  using Max = __half;
+  OGB_DEVICE static __half2 two(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+  OGB_DEVICE static float max_of(const uint32_t (&w)[8]) {
+    __half2 m = two(w[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = __hmax2(m, two(w[j]));
+    const float2 f = __half22float2(m);
+    return fmaxf(f.x, f.y);
+  }
+  template <typename F>
+  OGB_DEVICE static void pairs(const uint32_t (&w)[8], F&& f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 t = __half22float2(two(w[j]));
+      f(Float2(t.x, t.y));
+    }
+  }
+  OGB_DEVICE static int above(const uint32_t (&w)[8], float given) {
+    const __half2 g = __float2half2_rn(given);
+    __half2 n = __hgt2(two(w[0]), g);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) n = __hadd2(n, __hgt2(two(w[j]), g));
+    const float2 f = __half22float2(n);
+    return static_cast<int>(f.x + f.y);
+  }
+  OGB_DEVICE static float value(const uint32_t (&w)[8], int j) {
+    const float2 t = __half22float2(two(w[j >> 1]));
+    return (j & 1) != 0 ? t.y : t.x;
+  }
+  static constexpr uint32_t kNothing = 0xfc00fc00u;
+};
+OGB_DEVICE float lp_float(float v) { return v; }
+OGB_DEVICE float lp_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+OGB_DEVICE float lp_float(__half v) { return __half2float(v); }
 
 template <typename T>
 struct LpShared {
-  static constexpr int kPiece = LpType<T>::kPer * kLpBlocks;          // values of a thread in a round
-  static constexpr int kMost = kLpMaxTop * kPiece + kLpMaxTop;
-  unsigned long long keys[kMost];                 // the best so far, and behind them what a round added
-  unsigned long long best[kLpThreads];            // of each thread in a round; then the list in order
+  static constexpr int kPer = LpType<T>::kPer;
+  static constexpr int kMost = (kLpMaxTop > kLpQuick ? kLpMaxTop : kLpQuick) * kPer + kLpMaxTop;
+  __align__(16) unsigned long long keys[kMost + 8];           // the best so far, behind them what was added, and zeros to a multiple of eight
+  __align__(16) unsigned long long best[kLpThreads];          // of each thread; then the list in order
   unsigned long long bound;
   LpState part[kLpWarps];
   int rank_part[kLpWarps];
-  int count;
+  int count, reach;
   LpState total;
   int rank_total;
 };
 
-// The place of `key` among n keys in shared memory: how many are above it.
+// The place of `key` among n keys in shared memory, n a multiple of eight: how many are above it.
 OGB_DEVICE int lp_place(const unsigned long long* keys, int n, unsigned long long key) {
   int above = 0;
-  for (int i = 0; i < n; ++i) above += keys[i] > key ? 1 : 0;
+  for (int i = 0; i < n; i += 8) {
+    ulonglong2 k[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const ulonglong2*>(keys + i + 2 * j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) above += (k[j].x > key ? 1 : 0) + (k[j].y > key ? 1 : 0);
+  }
   return above;
 }
 
-template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobsParams p) {
+// The piece of a row of `vocab` logits that begins at value i0 (below zero or past the end where the row's ends are not at multiples of 32 bytes).
+template <typename T>
+OGB_DEVICE void lp_load(const T* x, int i0, int vocab, uint32_t (&w)[8]) {
   using Type = LpType<T>;
-  constexpr int kPer = Type::kPer;
+  if (i0 >= 0 && i0 + Type::kPer <= vocab) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(x + i0));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w[j] = Type::kNothing;
+    if constexpr (Type::kPer == 8) {
+      if (i0 + j >= 0 && i0 + j < vocab) w[j] = __float_as_uint(x[i0 + j]);
+    } else {
+      const int i = i0 + 2 * j;
+      const uint16_t* s = reinterpret_cast<const uint16_t*>(x);
+      if (i >= 0 && i < vocab) w[j] = (w[j] & 0xffff0000u) | s[i];
+      if (i + 1 >= 0 && i + 1 < vocab) w[j] = (w[j] & 0xffffu) | static_cast<uint32_t>(s[i + 1]) << 16;
+    }
+  }
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobsParams p) {
+  using Type = LpType<T>;
+  constexpr int kPer = Type::kPer, kUnroll = TOP ? 2 : 4;       // 32-byte pieces that a thread has in flight, as registers allow
   __shared__ LpShared<T> sh;
+  extern __shared__ __align__(16) uint8_t dynamic_smem[];
+  typename Type::Max* piece_max = reinterpret_cast<typename Type::Max*>(dynamic_smem);
   const int split = p.splits > 1 ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
   const int row = blockIdx.x / p.splits, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x = static_cast<const T*>(p.logits) + static_cast<size_t>(row) * p.ld;
@@ -107,125 +236,169 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobsPara
   const bool known = token >= 0 && token < p.vocab;
   const float given = known ? load_elem(x, Type::kElem, token) : INFINITY;
 
-  // 16-byte blocks that the row touches; those it does not fill (its ends, where it is not aligned) are read value by value
-  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int blocks = (off + p.vocab + kPer - 1) / kPer;
-  const int each = (blocks + p.splits - 1) / p.splits;
-  const int b0 = split * each, b1 = min(blocks, b0 + each);
-  const uint4* base = reinterpret_cast<const uint4*>(x - off);
-  auto load = [&](int b, float (&f)[kPer]) {
-    const int i0 = b * kPer - off;
-    if (b < b1 && i0 >= 0 && i0 + kPer <= p.vocab) {
-      const uint4 v = __ldcs(base + b);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kPer == 4) {
-          f[j] = __uint_as_float(w[j]);
-        } else {
-          const float2 t = Type::kElem == kElemBf16 ? unpack_bf16(w[j]) : __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          f[2 * j] = t.x;
-          f[2 * j + 1] = t.y;
-        }
-      }
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) f[j] = b < b1 && i0 + j >= 0 && i0 + j < p.vocab ? load_elem(x, Type::kElem, i0 + j) : -INFINITY;
-  };
+  // 32-byte pieces that the row touches, an equal share of them to every CTA of the cluster
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 31) / sizeof(T));
+  const int pieces = (off + p.vocab + kPer - 1) / kPer;
+  const int each = (pieces + p.splits - 1) / p.splits;
+  const int b0 = min(pieces, split * each), n_pieces = min(pieces, b0 + each) - b0;
+  const int first = b0 * kPer - off;                        // value at which this CTA's share begins
+  auto is_edge = [&](int i0) { return i0 < 0 || i0 + kPer > p.vocab; };
 
-  LpState st{-INFINITY, 0.f, 0.f};
+  // ---- the pass ----
+  float ref = -INFINITY, neg = 0.f;                         // m; minus m, zero as long as there is no value
+  Float2 s2(0.f), t2(0.f);
   int rank = 0;
-  unsigned long long floor_key = 0;      // nothing at or below it is among the best
-  float floor_value = -INFINITY;
-  int held = 0;                          // keys in the list
-  if (TOP && tid == 0) sh.count = 0;
-  if (TOP) __syncthreads();
-
-  for (int b = b0; b < b1; b += kLpThreads * kLpBlocks) {
-    float f[kLpBlocks][kPer];
+  const Float2 log2e(1.4426950408889634f);
+  for (int b = tid; b < n_pieces; b += kLpThreads * kUnroll) {
+    uint32_t w[kUnroll][8];
 #pragma unroll
-    for (int u = 0; u < kLpBlocks; ++u) load(b + u * kLpThreads + tid, f[u]);
-    float top = f[0][0];
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u * kLpThreads < n_pieces) lp_load(x, first + (b + u * kLpThreads) * kPer, p.vocab, w[u]);
 #pragma unroll
-    for (int u = 0; u < kLpBlocks; ++u)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) top = fmaxf(top, f[u][j]);
-    if (top > st.m) {
-      if (st.m != -INFINITY) {
-        const float d = fmaxf(st.m - top, -1000.f), r = __expf(d);     // a type's lowest value is minus infinity apart, in effect
-        st.t = r * fmaf(d, st.s, st.t);
-        st.s *= r;
-      }
-      st.m = top;
-    }
-    const float m = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int u = 0; u < kLpBlocks; ++u)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float d = f[u][j] - m, e = __expf(d);
-        st.s += e;
-        if (ENTROPY) st.t = fmaf(e, fmaxf(d, -1000.f), st.t);
-        rank += f[u][j] > given ? 1 : 0;
-      }
-    if (TOP) {
-      unsigned long long mine = 0;
-      if (!(top < floor_value)) {
-#pragma unroll
-        for (int u = 0; u < kLpBlocks; ++u)
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const int i = (b + u * kLpThreads + tid) * kPer - off + j;
-            const unsigned long long key = b + u * kLpThreads + tid < b1 && i >= 0 && i < p.vocab ? lp_key(f[u][j], i) : 0;
-            mine = key > mine ? key : mine;
+    for (int u = 0; u < kUnroll; ++u) {
+      const int piece = b + u * kLpThreads;
+      if (piece < n_pieces) {
+        const float top = Type::max_of(w[u]);
+        if (top - ref > kLpSlack || (ref == -INFINITY && top > -INFINITY)) {
+          if (ref != -INFINITY) {
+            const float d = fmaxf(ref - top, -1000.f);      // a type's lowest value is minus infinity apart, in effect
+            const Float2 r(__expf(d));
+            t2 = r * fma2(Float2(d), s2, t2);
+            s2 = r * s2;
           }
-        if (mine <= floor_key) mine = 0;
-      }
-      const int threads = __syncthreads_count(mine != 0);
-      if (threads == 0) continue;
-      if (threads > p.top) {
-        sh.best[tid] = mine;
-        __syncthreads();
-        const int place = mine != 0 ? lp_place(sh.best, kLpThreads, mine) : kLpThreads;
-        if (place == p.top - 1) sh.bound = mine;
-        __syncthreads();
-        floor_key = sh.bound - 1;                                    // the bound itself is kept
-      }
-      if (mine > floor_key) {
-#pragma unroll
-        for (int u = 0; u < kLpBlocks; ++u)
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const int i = (b + u * kLpThreads + tid) * kPer - off + j;
-            if (b + u * kLpThreads + tid < b1 && i >= 0 && i < p.vocab) {
-              const unsigned long long key = lp_key(f[u][j], i);
-              if (key > floor_key) sh.keys[held + atomicAdd(&sh.count, 1)] = key;
-            }
-          }
-      }
-      __syncthreads();
-      const int n = held + sh.count;
-      if (n >= p.top) {
-        for (int i = tid; i < n; i += kLpThreads) {
-          const unsigned long long key = sh.keys[i];
-          const int place = lp_place(sh.keys, n, key);
-          if (place < p.top) sh.best[place] = key;
+          ref = top;
+          neg = -top;
         }
-        __syncthreads();
-        if (tid < p.top) sh.keys[tid] = sh.best[tid];
-        held = p.top;
-        floor_key = sh.best[p.top - 1];
-        floor_value = lp_value(floor_key);
-      } else {
-        held = n;
+        const Float2 minus(neg);
+        Type::pairs(w[u], [&](Float2 v) {
+          const Float2 d = v + minus, a = d * log2e;
+          const Float2 e(ex2_approx(a.lo()), ex2_approx(a.hi()));
+          s2 = s2 + e;
+          if (ENTROPY) t2 = fma2(e, Float2(fmaxf(d.lo(), -1000.f), fmaxf(d.hi(), -1000.f)), t2);
+        });
+        if (top > given) rank += Type::above(w[u], given);
+        if (TOP) {
+          float kept = top;
+          const int i0 = first + piece * kPer;
+          if (is_edge(i0)) {                                // without what is not there
+            kept = __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              if (i0 + j >= 0 && i0 + j < p.vocab) kept = fmaxf(kept, Type::value(w[u], j));
+          }
+          if constexpr (Type::kElem == kElemF32) piece_max[piece] = kept;
+          else if constexpr (Type::kElem == kElemBf16) piece_max[piece] = __float2bfloat16(kept);
+          else piece_max[piece] = __float2half_rn(kept);
+        }
       }
-      if (tid == 0) sh.count = 0;
+    }
+  }
+  LpState st{ref, s2.lo() + s2.hi(), t2.lo() + t2.hi()};
+
+  // ---- the likeliest of this CTA's share, and perhaps some more, kLpMaxTop of them at most, at the head of sh.keys ----
+  int held = 0;
+  if (TOP) {
+    // the best key of a piece is at most that of its maximum at its first value, at least that at its last
+    auto upper = [&](int piece) { return lp_key(lp_float(piece_max[piece]), max(0, first + piece * kPer)); };
+    auto add_piece = [&](int piece, unsigned long long floor_key) {
+      uint32_t w[8];
+      const int i0 = first + piece * kPer;
+      lp_load(x, i0, p.vocab, w);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (i0 + j >= 0 && i0 + j < p.vocab) {
+          const unsigned long long key = lp_key(Type::value(w, j), i0 + j);
+          if (key > floor_key) sh.keys[held + atomicAdd(&sh.count, 1)] = key;
+        }
+    };
+    // keeps the best of held + count keys; the least of them when there are enough, else the floor as it was
+    auto keep_best = [&](unsigned long long floor_key) {
+      const int n = held + sh.count, padded = (n + 7) / 8 * 8;
+      if (tid < padded - n) sh.keys[n + tid] = 0;
       __syncthreads();
+      for (int i = tid; i < n; i += kLpThreads) {
+        const unsigned long long key = sh.keys[i];
+        const int place = lp_place(sh.keys, padded, key);
+        if (place < p.top) sh.best[place] = key;
+      }
+      __syncthreads();
+      held = min(n, p.top);
+      if (tid < held) sh.keys[tid] = sh.best[tid];
+      if (tid == 0) sh.count = 0;
+      if (n >= p.top) floor_key = sh.best[p.top - 1];
+      __syncthreads();
+      return floor_key;
+    };
+    float best = -INFINITY;
+    int best_piece = -1;
+    for (int b = tid; b < n_pieces; b += kLpThreads) {
+      const float m = lp_float(piece_max[b]);
+      if (m > best || (best_piece < 0 && m == m)) { best = m; best_piece = b; }      // nothing but NaN: no bound from this thread
+    }
+    unsigned long long own_best = best_piece >= 0 ? lp_key(best, min(p.vocab - 1, first + best_piece * kPer + kPer - 1)) : 0;
+    // where every thread has several pieces, four threads' best is bound enough, and 64 keys take a sixteenth of the comparisons
+    const int group = n_pieces >= 2 * kLpThreads ? 4 : 1;
+    if (group == 4) {
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, own_best, o);
+        own_best = other > own_best ? other : own_best;
+      }
+    }
+    if (tid % group == 0) sh.best[tid / group] = own_best;
+    if (tid == 0) { sh.count = 0; sh.reach = 0; sh.bound = 0; }
+    __syncthreads();
+    if (tid % group == 0 && own_best != 0 && lp_place(sh.best, kLpThreads / group, own_best) == p.top - 1) sh.bound = own_best;
+    __syncthreads();
+    unsigned long long floor_key = sh.bound != 0 ? sh.bound - 1 : 0;          // fewer threads than `top` have a value: every value may be one
+    const float floor_value = lp_value(floor_key + 1);
+    auto reaches = [&](int b) { return !(lp_float(piece_max[b]) < floor_value) && upper(b) > floor_key; };
+    int mine = 0;
+    for (int b = tid; b < n_pieces; b += kLpThreads) mine += reaches(b) ? 1 : 0;
+    if (mine != 0) atomicAdd(&sh.reach, mine);
+    __syncthreads();
+    if (sh.reach <= kLpQuick) {
+      for (int b = tid; mine != 0; b += kLpThreads)
+        if (reaches(b)) {
+          add_piece(b, floor_key);
+          --mine;
+        }
+      __syncthreads();
+      if (sh.count <= kLpMaxTop) held = sh.count;           // the join puts them in order
+      else keep_best(floor_key);
+    } else {
+      for (int b = 0; b < n_pieces; b += kLpThreads) {
+        // a round: a piece a thread.  At most `top` threads keep one whose best key reaches the bound of this round.
+        bool in = b + tid < n_pieces && upper(b + tid) > floor_key;
+        const int threads = __syncthreads_count(in);
+        if (threads == 0) continue;
+        unsigned long long own = 0;
+        if (in) {
+          uint32_t w[8];
+          const int i0 = first + (b + tid) * kPer;
+          lp_load(x, i0, p.vocab, w);
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            if (i0 + j >= 0 && i0 + j < p.vocab) {
+              const unsigned long long key = lp_key(Type::value(w, j), i0 + j);
+              own = key > own ? key : own;
+            }
+          if (own <= floor_key) own = 0;
+        }
+        sh.best[tid] = own;
+        if (tid == 0) sh.bound = 0;
+        __syncthreads();
+        if (own != 0 && lp_place(sh.best, kLpThreads, own) == p.top - 1) sh.bound = own;
+        __syncthreads();
+        if (sh.bound != 0) floor_key = sh.bound - 1;
+        if (own > floor_key) add_piece(b + tid, floor_key);
+        __syncthreads();
+        floor_key = keep_best(floor_key);
+      }
     }
   }
 
-  // threads -> warps -> the CTA
+  // ---- threads -> warps -> the CTA ----
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const LpState other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
@@ -249,14 +422,23 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobsPara
     st = sh.total;
     rank = sh.rank_total;
     int n = held;
-    for (int r = 1; r < p.splits; ++r) {
-      const LpShared<T>& peer = *cg::this_cluster().map_shared_rank(&sh, r);
-      st = lp_join(st, peer.total);
-      rank += peer.rank_total;
-      if (TOP) {
-        const int more = peer.count;
-        if (tid < more) sh.keys[n + tid] = peer.keys[tid];
-        n += more;
+    if (p.splits > 1) {
+      const LpShared<T>& peer = *cg::this_cluster().map_shared_rank(&sh, min(lane, p.splits - 1));
+      const LpState theirs = peer.total;
+      const int their_rank = peer.rank_total, their_count = TOP ? peer.count : 0;
+      n = 0;
+      int base = 0;                                          // the list of CTA r goes behind those before it, a warp a CTA
+#pragma unroll
+      for (int r = 0; r < kLpMaxSplit; ++r) {
+        const LpState other{__shfl_sync(0xffffffffu, theirs.m, r), __shfl_sync(0xffffffffu, theirs.s, r), __shfl_sync(0xffffffffu, theirs.t, r)};
+        const int more = __shfl_sync(0xffffffffu, their_rank, r), count = __shfl_sync(0xffffffffu, their_count, r);
+        if (r == warp) base = n;
+        if (r < p.splits) n += count;
+        if (r > 0 && r < p.splits) { st = lp_join(st, other); rank += more; }
+      }
+      if (TOP && warp > 0 && warp < p.splits) {
+        const LpShared<T>& from = *cg::this_cluster().map_shared_rank(&sh, warp);
+        if (lane < __shfl_sync(0xffffffffu, their_count, warp)) sh.keys[base + lane] = from.keys[lane];
       }
     }
     const float log_s = logf(st.s);
@@ -267,14 +449,14 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobsPara
       if (ENTROPY) p.entropy[row] = log_s - st.t / st.s;
     }
     if (TOP) {
+      const int padded = (n + 7) / 8 * 8;
+      if (tid < padded - n) sh.keys[n + tid] = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += kLpThreads) {
-        const unsigned long long key = sh.keys[i];
-        const int place = lp_place(sh.keys, n, key);
-        if (place < p.top) {
-          p.top_ids[static_cast<size_t>(row) * p.top + place] = lp_index(key);
-          p.top_logprob[static_cast<size_t>(row) * p.top + place] = lp_value(key) - st.m - log_s;
-        }
+      const unsigned long long key = tid < n ? sh.keys[tid] : 0;
+      const int place = key != 0 ? lp_place(sh.keys, padded, key) : p.top;
+      if (place < p.top) {
+        p.top_ids[static_cast<size_t>(row) * p.top + place] = lp_index(key);
+        p.top_logprob[static_cast<size_t>(row) * p.top + place] = lp_value(key) - st.m - log_s;
       }
     }
   }
@@ -283,11 +465,23 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobsPara
 
 template <typename T>
 static int launch_logprobs(const LogprobsParams& p, cudaStream_t stream) {
+  constexpr int kPer = LpType<T>::kPer;
+  static OncePerDevice allowed[2];
+  int smem = 0;
+  if (p.top > 0) {
+    const long long pieces = (static_cast<long long>(p.vocab) + 2 * kPer - 2) / kPer;
+    const long long bytes = ((pieces + p.splits - 1) / p.splits * static_cast<long long>(sizeof(typename LpType<T>::Max)) + 15) / 16 * 16;
+    if (bytes > kLpSmem) return -9;
+    smem = static_cast<int>(bytes);
+    const int rc = p.entropy != nullptr ? allow_smem(allowed[0], logprobs_kernel<T, true, true>, kLpSmem) : allow_smem(allowed[1], logprobs_kernel<T, false, true>, kLpSmem);
+    if (rc != 0) return rc;
+  }
   auto kernel = p.top > 0 ? (p.entropy != nullptr ? logprobs_kernel<T, true, true> : logprobs_kernel<T, false, true>)
                           : (p.entropy != nullptr ? logprobs_kernel<T, true, false> : logprobs_kernel<T, false, false>);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.splits);
   cfg.blockDim = dim3(kLpThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -310,9 +504,10 @@ extern "C" int ogb_token_logprobs(const void* logits, const int* tokens, float* 
   if (vocab > (1 << 30) || rows > (1 << 28)) return -2;
   LogprobsParams p{logits, tokens, logprob, entropy, top_logprob, rank, top_ids, ld, rows, vocab, top, 1, status};
   const int sms = ogb_num_sms();
-  // parts of a row: until every SM has work, as long as a part keeps a round's worth of values
-  const int round = kLpThreads * kLpBlocks * 16 / elem_bytes(elem);
-  while (p.splits < kLpMaxSplit && static_cast<long long>(rows) * p.splits < sms && static_cast<long long>(p.splits) * round < vocab) p.splits *= 2;
+  // parts of a row: until every SM has a few CTAs, as long as each keeps a piece or so a thread; more where the maxima of its pieces would not fit
+  const long long round = kLpThreads * 32 / elem_bytes(elem);
+  const long long fits = static_cast<long long>(kLpSmem) * 32 / elem_bytes(elem) / elem_bytes(elem) - 64;
+  while (p.splits < kLpMaxSplit && ((static_cast<long long>(rows) * p.splits < 2 * sms && p.splits * round < vocab) || (top > 0 && p.splits * fits < vocab))) p.splits *= 2;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (elem == kElemF32) return launch_logprobs<float>(p, stream);
   if (elem == kElemBf16) return launch_logprobs<__nv_bfloat16>(p, stream);

@@ -555,6 +555,7 @@ class TokenLogprobs(NamedTuple):
 
 _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_TOP_LOGPROBS = 32
+MAX_VOCAB, MAX_VOCAB_WITH_TOP = 1 << 30, 3_000_000
 
 
 @_timed("token_logprobs")
@@ -570,6 +571,8 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
     rows, vocab = logits.shape
     if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):
         raise ValueError(f"top = {top}: between 0 and {min(MAX_TOP_LOGPROBS, vocab)}")
+    if vocab > MAX_VOCAB or (top and vocab > MAX_VOCAB_WITH_TOP):
+        raise ValueError(f"a vocabulary of {vocab}: at most {MAX_VOCAB_WITH_TOP if top else MAX_VOCAB}")
     if tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
         raise ValueError(f"tokens: {rows} whole numbers (int32, int64) on the device of the logits")
     if not logits.is_cuda:
