@@ -32,10 +32,13 @@ namespace ogb {
 int make_tmap_u8_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols);
 
 constexpr int kI8K = 128;                    // 128 bytes: a row of the 128-byte swizzle
-constexpr int kI8Threads = 192;
+constexpr int kI8Threads = 320;              // TMA, MMA, two groups of four epilogue warps
 constexpr int kI8MaxK = 131072;
 constexpr int kI8Group = 16;                 // tiles of W that go together against all rows
-constexpr int kI8Stage = 32 * 128 * 4;       // staging of 32 rows of an accumulator
+constexpr int kI8Groups = 2;                 // of epilogue warps, every other chunk of a tile's rows each
+template <int TW>
+constexpr int kI8Chunk = 32 / TW;            // rows of a chunk: 16 KB of sums, of both accumulators
+constexpr int kI8Stage = 32 * 128 * 4;       // staging of a group
 
 struct Int8Params {
   void* out;
@@ -48,7 +51,8 @@ struct Int8Params {
   int M, N, mn;                              // mn: rows of a tile, a multiple of 16
   int n_tiles, m_tiles, tiles, k_blocks, stages;
   int splits;                                // CTAs (a cluster) per tile; 0: whole tiles and ranges
-  int cut;                                   // the first `cut` tiles are cut into ranges
+  int cut;                                   // the first `cut` tiles are cut into ranges of
+  int range, longer;                         //   `range` k-blocks a CTA, and one more for the first `longer`
   int* status;
   int* ws;                                   // [CTA][2][TW][4 quarters][rows / 4][32 channels][4 rows]
   unsigned int* counters;                    // [CTA], zero when the kernel starts
@@ -78,31 +82,44 @@ OGB_DEVICE void i8_tile(const Int8Params& p, int tile, int& nt, int& mt) {
   mt = t / wide;
 }
 
+// First k-block of a CTA's range, and the CTA whose range holds one.
+OGB_DEVICE int i8_range_begin(const Int8Params& p, int cta) { return cta * p.range + min(cta, p.longer); }
+OGB_DEVICE int i8_range_owner(const Int8Params& p, int i) {
+  const int edge = (p.range + 1) * p.longer;
+  return i < edge ? i / (p.range + 1) : p.longer + (i - edge) / p.range;
+}
+
 // The parts of tiles that a CTA computes, in order: of its range the tile it shares with the CTA before it, the one it shares with the CTA
-// after it and the whole ones; then its whole tiles.
+// after it and the whole ones; then its whole tiles.  (Fewer than 200 tiles of at most 1024 k-blocks are cut: 32 bits hold their sum.)
 struct Int8Segs {
-  long long it0, it1, first_end, last_begin, mid;
+  int it0, it1, first_end, last_begin, mid;
   int k_blocks, state = 0, tile, tiles, stride;
   OGB_DEVICE explicit Int8Segs(const Int8Params& p) : k_blocks(p.k_blocks), tiles(p.tiles) {
     stride = gridDim.x;
     if (p.splits > 0) {
-      const long long base = static_cast<long long>(blockIdx.x / p.splits) * k_blocks;
-      const int rank = blockIdx.x % p.splits;
-      it0 = base + k_blocks * rank / p.splits;
-      it1 = base + k_blocks * (rank + 1) / p.splits;
+      // one part of one tile, which `mid` finds whole
+      const int t = blockIdx.x / p.splits, rank = blockIdx.x - t * p.splits;
+      it0 = t * k_blocks + k_blocks * rank / p.splits;
+      it1 = t * k_blocks + k_blocks * (rank + 1) / p.splits;
+      first_end = it1;
+      last_begin = mid = it1;
       tile = tiles;
-    } else {
-      const long long total = static_cast<long long>(p.cut) * k_blocks;
-      it0 = GemmWork::range_begin(total, gridDim.x, blockIdx.x);
-      it1 = GemmWork::range_begin(total, gridDim.x, blockIdx.x + 1);
-      tile = p.cut + blockIdx.x;
+      return;
     }
-    first_end = it0 % k_blocks != 0 ? min(it1, (it0 / k_blocks + 1) * k_blocks) : it0;
-    last_begin = it1 % k_blocks != 0 ? max(first_end, it1 / k_blocks * k_blocks) : it1;
+    tile = p.cut + blockIdx.x;
+    it0 = i8_range_begin(p, blockIdx.x);
+    it1 = i8_range_begin(p, blockIdx.x + 1);
+    first_end = it0;
+    last_begin = it1;
+    if (it1 > it0) {
+      const int t0 = it0 / k_blocks, t1 = it1 / k_blocks;
+      if (it0 != t0 * k_blocks) first_end = min(it1, (t0 + 1) * k_blocks);
+      if (it1 != t1 * k_blocks) last_begin = max(first_end, t1 * k_blocks);
+    }
     mid = first_end;
   }
   OGB_DEVICE bool next(int& t, int& kb0, int& kb1) {
-    long long a = 0, b = 0;
+    int a = 0, b = 0;
     if (state == 0) { a = it0; b = first_end; state = 1; }
     if (state == 1 && a >= b) { a = last_begin; b = it1; state = 2; }
     if (state == 2 && a >= b) {
@@ -116,9 +133,9 @@ struct Int8Segs {
         return true;
       }
     }
-    t = static_cast<int>(a / k_blocks);
-    kb0 = static_cast<int>(a - static_cast<long long>(t) * k_blocks);
-    kb1 = static_cast<int>(b - static_cast<long long>(t) * k_blocks);
+    t = a / k_blocks;
+    kb0 = a - t * k_blocks;
+    kb1 = b - t * k_blocks;
     return true;
   }
 };
@@ -139,29 +156,37 @@ struct Int8Cursor {
   }
 };
 
-// What a lane needs of its four neighbouring channels, for all rows of a tile.
+// What a lane needs of its four channels for all rows of a tile: neighbouring ones, or where rows of the result are not at multiples of four values
+// every 32nd, so that a warp stores neighbours together.
 template <int TW>
 struct Int8Channels {
-  int n, n_out;                               // first column of the result, and how many there are
+  int n, step, n_out;                         // first column of the result, way to the next, and how many there are
   float c[TW][4], b[TW][4];
   OGB_DEVICE Int8Channels(const Int8Params& p, int nt) {
     const int lane = threadIdx.x & 31;
-    n = nt * 128 + 4 * lane;
+    step = p.vec != 0 ? 1 : 32;
+    n = nt * 128 + (p.vec != 0 ? 4 * lane : lane);
     n_out = p.N / TW;
 #pragma unroll
     for (int w = 0; w < TW; ++w)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = min((nt * TW + w) * 128 + 4 * lane + i, p.N - 1);
+        const int at = min((nt * TW + w) * 128 + n - nt * 128 + i * step, p.N - 1);
         c[w][i] = __ldg(p.channel + at);
         b[w][i] = p.bias != nullptr ? __ldg(p.bias + at) : 0.f;
       }
+  }
+  // a lane's four sums of a row of 128
+  OGB_DEVICE int4 sums(const int* row) const {
+    const int lane = threadIdx.x & 31;
+    if (step == 1) return *reinterpret_cast<const int4*>(row + 4 * lane);
+    return make_int4(row[lane], row[lane + 32], row[lane + 64], row[lane + 96]);
   }
 };
 // Sums of row m (and of the up half) -> the stored result.
 template <int TW>
 OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m, float s, const int4& a, const int4& u) {
-  if (ch.n >= ch.n_out) return;
+  if (ch.n >= ch.n_out) return;                               // the others are further on
   const int raw[4] = {a.x, a.y, a.z, a.w}, up[4] = {u.x, u.y, u.z, u.w};
   float v[4];
 #pragma unroll
@@ -193,16 +218,38 @@ OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m,
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (ch.n + i < ch.n_out) store_elem(p.out, p.out_elem, at + i, p.residual != nullptr ? v[i] + load_elem(p.residual, p.out_elem, from + i) : v[i]);
+  for (int i = 0; i < 4; ++i) {
+    const int j = i * ch.step;
+    if (ch.n + j < ch.n_out) store_elem(p.out, p.out_elem, at + j, p.residual != nullptr ? v[i] + load_elem(p.residual, p.out_elem, from + j) : v[i]);
+  }
 }
 
-// The epilogue warps, where whole tiles and ranges are computed.
+// 32 lanes x 32 / TW consecutive columns of an accumulator
 template <int TW>
-OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars, int* stage) {
-  const int q = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const long long total = static_cast<long long>(p.cut) * p.k_blocks;
+OGB_DEVICE void i8_tmem_ld(uint32_t addr, uint32_t (&r)[kI8Chunk<TW>]) {
+  if constexpr (TW == 1) {
+    tmem_ld_32x32(addr, r);
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+  }
+}
+// Barriers of the epilogue warps: all of them, or a group's.
+OGB_DEVICE void i8_epi_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+OGB_DEVICE void i8_group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
+
+// The epilogue warps, where whole tiles and ranges are computed.  Warp index mod 4: the quarter of TMEM's lanes, 32 channels of a tile; each of the
+// two groups takes every other chunk of rows.
+template <int TW>
+OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars, int* staging) {
+  constexpr int kChunk = kI8Chunk<TW>;
+  const int warp = (threadIdx.x >> 5) - 2, q = (threadIdx.x >> 5) & 3, group = warp >> 2, lane = threadIdx.x & 31;
   const int slot = TW * 4 * acc_cols * 32;
+  int* stage = staging + group * (kI8Stage / 4);
   volatile int* abort_flag = &bars->abort_flag;
   volatile uint32_t* shared_last = &bars->shared_last;
   pdl_wait();
@@ -216,7 +263,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     const uint32_t buf_phase = (bufs == 2 ? seg >> 1 : seg) & 1;
     int nt, mt;
     i8_tile(p, tile, nt, mt);
-    const int rows = min(p.mn, p.M - mt * p.mn);
+    const int row0 = mt * p.mn, rows = min(p.mn, p.M - row0);
     // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out the warps go on
     // to arrive on the counters of their shared tiles.
     if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[buf], buf_phase))) {
@@ -227,79 +274,92 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * TW * acc_cols;
     int c_lo = 0, c_hi = 0;                                   // the CTAs that share the tile
     if (!whole) {
-      c_lo = GemmWork::owner(total, gridDim.x, static_cast<long long>(tile) * p.k_blocks);
-      c_hi = GemmWork::owner(total, gridDim.x, static_cast<long long>(tile + 1) * p.k_blocks - 1) + 1;
+      c_lo = i8_range_owner(p, tile * p.k_blocks);
+      c_hi = i8_range_owner(p, (tile + 1) * p.k_blocks - 1) + 1;
       if (ok) {
         int4* dst = reinterpret_cast<int4*>(p.ws + static_cast<size_t>(blockIdx.x * 2 + (head ? 1 : 0)) * slot) + q * acc_cols * 8 + lane;
 #pragma unroll
         for (int w = 0; w < TW; ++w) {
 #pragma unroll 1
-          for (int c = 0; c < rows; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32(t_addr + w * acc_cols + c, r);
+          for (int c = group * kChunk; c < rows; c += kI8Groups * kChunk) {
+            uint32_t r[kChunk];
+            i8_tmem_ld<TW>(t_addr + w * acc_cols + c, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
+            for (int j = 0; j < kChunk; j += 4)
               if (c + j < rows) __stcg(dst + (w * 4 * acc_cols + c + j) * 8, make_int4(r[j], r[j + 1], r[j + 2], r[j + 3]));
           }
         }
       }
       tc_fence_before();
       __threadfence();
-      rows_epi_sync();
+      i8_epi_sync();
       if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
-      if (q == 0 && lane == 0) {
+      if (warp == 0 && lane == 0) {
         *shared_last = atomicAdd(p.counters + c_lo, 1u) == static_cast<unsigned int>(c_hi - c_lo - 1);
         __threadfence();
       }
-      rows_epi_sync();
+      i8_epi_sync();
       const bool last = *shared_last != 0;
-      rows_epi_sync();
+      i8_epi_sync();
       if (!__all_sync(0xffffffffu, ok && last)) continue;
     } else if (!ok) {
       continue;
     }
     const Int8Channels<TW> ch(p, nt);
+    // the factors of a chunk's rows, a lane each
+    auto chunk_factor = [&](int c) { return lane < kChunk && c + lane < rows ? factor[row0 + c + lane] : 0.f; };
+    float f = chunk_factor(group * kChunk);
 #pragma unroll 1
-    for (int c = 0; c < rows; c += 32) {
+    for (int c = group * kChunk; c < rows; c += kI8Groups * kChunk) {
+      const float f_next = chunk_factor(c + kI8Groups * kChunk);
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
-        int v[32];
+        int v[kChunk];
         if (whole) {
-          uint32_t r[32];
-          tmem_ld_32x32(t_addr + w * acc_cols + c, r);
+          uint32_t r[kChunk];
+          i8_tmem_ld<TW>(t_addr + w * acc_cols + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
+          for (int j = 0; j < kChunk; ++j) v[j] = static_cast<int>(r[j]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0;
+          for (int j = 0; j < kChunk; ++j) v[j] = 0;
+          // two CTAs at a time
 #pragma unroll 1
-          for (int x = c_lo; x < c_hi; ++x) {
-            // the first CTA of a tile holds its head (slot 1), the others a later part (slot 0)
-            const int4* src = reinterpret_cast<const int4*>(p.ws + static_cast<size_t>(x * 2 + (x == c_lo ? 1 : 0)) * slot) + ((w * 4 + q) * acc_cols + c) * 8 + lane;
-            int4 t[8];
+          for (int x = c_lo; x < c_hi; x += 2) {
+            int4 t[2][kChunk / 4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = __ldcg(src + j * 32);
+            for (int i = 0; i < 2; ++i) {
+              // the first CTA of a tile holds its head (slot 1), the others a later part (slot 0)
+              const int from = min(x + i, c_hi - 1);
+              const int4* src = reinterpret_cast<const int4*>(p.ws + static_cast<size_t>(from * 2 + (from == c_lo ? 1 : 0)) * slot) +
+                                ((w * 4 + q) * acc_cols + c) * 8 + lane;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[4 * j] += t[j].x; v[4 * j + 1] += t[j].y; v[4 * j + 2] += t[j].z; v[4 * j + 3] += t[j].w; }
+              for (int j = 0; j < kChunk / 4; ++j) t[i][j] = __ldcg(src + j * 32);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (x + i < c_hi) {
+#pragma unroll
+                for (int j = 0; j < kChunk / 4; ++j) {
+                  v[4 * j] += t[i][j].x; v[4 * j + 1] += t[i][j].y; v[4 * j + 2] += t[i][j].z; v[4 * j + 3] += t[i][j].w;
+                }
+              }
           }
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) stage[(w * 32 + j) * 128 + q * 32 + lane] = v[j];
+        for (int j = 0; j < kChunk; ++j) stage[(w * kChunk + j) * 128 + q * 32 + lane] = v[j];
       }
-      rows_epi_sync();
+      i8_group_sync(group);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int m = q * 8 + j;
-        if (c + m < rows) {
-          const int row = mt * p.mn + c + m;
-          const int4 a = *reinterpret_cast<const int4*>(stage + m * 128 + 4 * lane);
-          const int4 u = *reinterpret_cast<const int4*>(stage + ((TW - 1) * 32 + m) * 128 + 4 * lane);
-          i8_store<TW>(p, ch, row, factor[row], a, u);
-        }
+      for (int j = 0; j < kChunk / 4; ++j) {
+        const int m = q * (kChunk / 4) + j;
+        const float s = __shfl_sync(0xffffffffu, f, m);
+        if (c + m < rows) i8_store<TW>(p, ch, row0 + c + m, s, ch.sums(stage + m * 128), ch.sums(stage + ((TW - 1) * kChunk + m) * 128));
       }
-      rows_epi_sync();
+      i8_group_sync(group);
+      f = f_next;
     }
     if (whole) {
       tc_fence_before();
@@ -312,6 +372,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
 // All threads of a CTA, after their parts of the main loop: the epilogue of a tile that a cluster shares.  smem: the ring, free by then.
 template <int TW>
 OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int acc_cols, RowsBars* bars, uint8_t* smem, int ring_bytes) {
+  constexpr int kChunk = kI8Chunk<TW>;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* stage = reinterpret_cast<int*>(smem);
   bool ok = true;
@@ -320,40 +381,59 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
   const int tile = blockIdx.x / p.splits, rank = blockIdx.x % p.splits;
   int nt, mt;
   i8_tile(p, tile, nt, mt);
-  const int rows = min(p.mn, p.M - mt * p.mn);
+  const int row0 = mt * p.mn, rows = min(p.mn, p.M - row0);
+  // Row k of those this warp will store is rank + splits * (warp + warps * k); their factors, a lane each, and the channels come while the
+  // products are still under way.
   const Int8Channels<TW> ch(p, nt);
+  const int first = rank + p.splits * warp, stride = p.splits * warps;
+  float f = first + stride * lane < rows ? factor[row0 + first + stride * lane] : 0.f;
   if (warp >= 2) {
     ok = __all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[0], 0));      // every product has retired: the ring is free
     if (!ok && lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1; }
     tc_fence_after();
-  }
-  const int most = ring_bytes / (TW * 512) / 32 * 32;
-  for (int r0 = 0; r0 < rows; r0 += most) {
-    const int count = min(most, (rows - r0 + 31) / 32 * 32);
-    if (warp >= 2 && ok) rows_lay_out<TW>(tmem_base, acc_cols, r0, count, reinterpret_cast<float*>(stage));
-    if (p.splits > 1) cooperative_groups::this_cluster().sync();
-    else __syncthreads();
-    for (int m = rank + p.splits * warp; m < count && r0 + m < rows; m += p.splits * warps) {
-      int4 s[TW];
+    if (ok) {
+      // all sums of the tile fit the ring: [accumulator][row][128]
+      const int q = warp & 3, group = (warp - 2) >> 2;
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
-        int4 t[kRowsMaxSplit];
-        const int* src = stage + (static_cast<size_t>(w) * count + m) * 128 + 4 * lane;
+#pragma unroll 1
+        for (int c = group * kChunk; c < rows; c += kI8Groups * kChunk) {
+          uint32_t r[kChunk];
+          i8_tmem_ld<TW>(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + w * acc_cols + c, r);
+          tmem_ld_wait();
+          int* dst = stage + (w * acc_cols + c) * 128 + q * 32 + lane;
 #pragma unroll
-        for (int x = 0; x < kRowsMaxSplit; ++x)
-          if (x < p.splits) t[x] = *reinterpret_cast<const int4*>(p.splits > 1 ? cooperative_groups::this_cluster().map_shared_rank(src, x) : src);
-        s[w] = t[0];
-#pragma unroll
-        for (int x = 1; x < kRowsMaxSplit; ++x)
-          if (x < p.splits) { s[w].x += t[x].x; s[w].y += t[x].y; s[w].z += t[x].z; s[w].w += t[x].w; }
+          for (int j = 0; j < kChunk; ++j) dst[j * 128] = static_cast<int>(r[j]);
+        }
       }
-      const int row = mt * p.mn + r0 + m;
-      i8_store<TW>(p, ch, row, factor[row], s[0], s[TW - 1]);
     }
-    // nobody overwrites or leaves what is being read
-    if (p.splits > 1) cooperative_groups::this_cluster().sync();
-    else __syncthreads();
   }
+  if (p.splits > 1) cooperative_groups::this_cluster().sync();
+  else __syncthreads();
+  int k = 0;
+#pragma unroll 2
+  for (int m = first; m < rows; m += stride, ++k) {
+    int4 s[TW];
+#pragma unroll
+    for (int w = 0; w < TW; ++w) {
+      const int* src = stage + (w * acc_cols + m) * 128;
+      if (p.splits == 1) {
+        s[w] = ch.sums(src);
+        continue;
+      }
+      int4 t[kRowsMaxSplit];
+#pragma unroll
+      for (int x = 0; x < kRowsMaxSplit; ++x)
+        if (x < p.splits) t[x] = ch.sums(cooperative_groups::this_cluster().map_shared_rank(src, x));
+      s[w] = t[0];
+#pragma unroll
+      for (int x = 1; x < kRowsMaxSplit; ++x)
+        if (x < p.splits) { s[w].x += t[x].x; s[w].y += t[x].y; s[w].z += t[x].z; s[w].w += t[x].w; }
+    }
+    i8_store<TW>(p, ch, row0 + m, __shfl_sync(0xffffffffu, f, k), s[0], s[TW - 1]);
+  }
+  // nobody leaves what is being read
+  if (p.splits > 1) cooperative_groups::this_cluster().sync();
 }
 
 template <int TW>
@@ -403,11 +483,37 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   const int bufs = p.splits == 0 && 2 * TW * acc_cols <= 512 ? 2 : 1;
   uint32_t tmem_cols = 32;
   while (static_cast<int>(tmem_cols) < bufs * TW * acc_cols) tmem_cols *= 2;
+  // The thread that issues the loads makes the barriers, and has the first ring of W on its way before anything else is set up -- and before
+  // the kernel ahead, which makes the rows, has ended.
+  int ahead = 0;
+  auto load_w = [&](const Int8Cursor& c, int st) {
+    mbar_expect_tx(&bars->full[st], stage_bytes);
+#pragma unroll
+    for (int w = 0; w < TW; ++w)
+      tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (c.nt * TW + w) * 128);
+  };
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmap_w);
-    tma_prefetch_desc(&tmap_q);
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->tmem_full[i], 1);
+      mbar_init(&bars->tmem_empty[i], 4 * kI8Groups);
+    }
+    bars->abort_flag = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
   }
-  const uint32_t tmem_base = rows_setup(bars, p.stages, 1, tmem_cols);
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_slot;
   pdl_trigger();
 
   if (warp == 0) {
@@ -416,15 +522,6 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      auto load_w = [&](const Int8Cursor& c, int st) {
-        mbar_expect_tx(&bars->full[st], stage_bytes);
-#pragma unroll
-        for (int w = 0; w < TW; ++w)
-          tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (c.nt * TW + w) * 128);
-      };
-      // the first ring of W is on its way before the kernel ahead, which makes the rows, has ended
-      int ahead = 0;
-      for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
       pdl_wait();
       for (Int8Cursor c(p); c.more; c.step()) {
         if (ahead > 0) {
@@ -473,7 +570,10 @@ static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
   r.k_blocks = (K + kI8K - 1) / kI8K;
   r.clusters = r.tiles <= sms;
   if (!r.clusters) {
-    r.cut = r.tiles % sms;
+    // The tiles of the incomplete last round; a round more where they are so few that many CTAs would share each of them (8 tiles, 18 CTAs
+    // each: one CTA then adds 18 partial sums of 128 KB).
+    const int rest = r.tiles % sms;
+    r.cut = rest == 0 ? 0 : 7 * rest < 2 * sms ? rest + sms : rest;
     if (r.cut > 0) {
       r.counter_bytes = (static_cast<long long>(sms) * 4 + 1023) / 1024 * 1024;
       r.ws_bytes = 2ll * sms * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
@@ -489,7 +589,7 @@ static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long l
   int rc = allow_smem(allowed, kernel, kRowsSmemMax);
   if (rc != 0) return rc;
   const int stage_bytes = TW * 128 * kI8K + p.mn * kI8K;
-  const int extra = kRowsBarBytes + (plan.clusters ? 0 : TW * kI8Stage);
+  const int extra = kRowsBarBytes + (plan.clusters ? 0 : kI8Groups * kI8Stage);
   p.stages = std::min(kRowsMaxStages, (kRowsSmemMax - extra) / stage_bytes);
   const int smem = p.stages * stage_bytes + extra;
   int grid = ogb_num_sms();
@@ -576,6 +676,6 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
   p.vec = (reinterpret_cast<uintptr_t>(out) % piece == 0 && ldc % 4 == 0 &&
            (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) % piece == 0 && ldr % 4 == 0))) ? 1 : 0;
   p.M = M; p.N = N; p.mn = plan.mn; p.n_tiles = plan.n_tiles; p.m_tiles = plan.m_tiles; p.tiles = plan.tiles; p.k_blocks = plan.k_blocks;
-  p.cut = plan.cut; p.status = status;
+  p.cut = plan.cut; p.range = plan.cut * plan.k_blocks / sms; p.longer = plan.cut * plan.k_blocks % sms; p.status = status;
   return gated != 0 ? launch_int8<2>(plan, p, q, ldq, w, ldw, K, early, stream) : launch_int8<1>(plan, p, q, ldq, w, ldw, K, early, stream);
 }
