@@ -183,9 +183,45 @@ struct Int8Channels {
     return make_int4(row[lane], row[lane + 32], row[lane + 64], row[lane + 96]);
   }
 };
+// A lane's four residuals of a row, fetched ahead of the sums they are added to.
+struct Int8Residual {
+  uint4 raw;
+  template <int TW>
+  OGB_DEVICE void load(const Int8Params& p, const Int8Channels<TW>& ch, int m) {
+    raw = make_uint4(0, 0, 0, 0);
+    if (p.residual == nullptr) return;
+    const size_t from = static_cast<size_t>(m) * p.ldr + ch.n;
+    if (p.vec != 0 && ch.n + 4 <= ch.n_out) {
+      if (p.out_elem == kElemF32) {
+        raw = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + from);
+      } else {
+        const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + from);
+        raw.x = r.x;
+        raw.y = r.y;
+      }
+      return;
+    }
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ch.n + i * ch.step < ch.n_out ? load_elem(p.residual, p.out_elem, from + i * ch.step) : 0.f;
+    // as the type's own bits again: what add() reads
+    if (p.out_elem == kElemF32) raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else if (p.out_elem == kElemBf16) raw = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), 0, 0);
+    else raw = make_uint4(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), 0, 0);
+  }
+  OGB_DEVICE void add(const Int8Params& p, float (&v)[4]) const {
+    if (p.out_elem == kElemF32) {
+      v[0] += __uint_as_float(raw.x); v[1] += __uint_as_float(raw.y); v[2] += __uint_as_float(raw.z); v[3] += __uint_as_float(raw.w);
+      return;
+    }
+    const float2 lo = p.out_elem == kElemBf16 ? unpack_bf16(raw.x) : __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+    const float2 hi = p.out_elem == kElemBf16 ? unpack_bf16(raw.y) : __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+    v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+  }
+};
 // Sums of row m (and of the up half) -> the stored result.
 template <int TW>
-OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m, float s, const int4& a, const int4& u) {
+OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m, float s, const int4& a, const int4& u, const Int8Residual& r) {
   if (ch.n >= ch.n_out) return;                               // the others are further on
   const int raw[4] = {a.x, a.y, a.z, a.w}, up[4] = {u.x, u.y, u.z, u.w};
   float v[4];
@@ -197,31 +233,19 @@ OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m,
       v[i] = __fdividef(v[i], 1.f + __expf(-v[i])) * w;
     }
   }
-  const size_t at = static_cast<size_t>(m) * p.ldc + ch.n, from = static_cast<size_t>(m) * p.ldr + ch.n;
+  if (TW == 1 && p.residual != nullptr) r.add(p, v);
+  const size_t at = static_cast<size_t>(m) * p.ldc + ch.n;
   if (p.vec != 0 && ch.n + 4 <= ch.n_out) {
-    if (p.out_elem == kElemF32) {
-      if (p.residual != nullptr) {
-        const float4 r = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + from);
-        v[0] += r.x; v[1] += r.y; v[2] += r.z; v[3] += r.w;
-      }
+    if (p.out_elem == kElemF32)
       *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-      return;
-    }
-    if (p.residual != nullptr) {
-      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + from);
-      const float2 lo = p.out_elem == kElemBf16 ? unpack_bf16(r.x) : __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-      const float2 hi = p.out_elem == kElemBf16 ? unpack_bf16(r.y) : __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-      v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
-    }
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = p.out_elem == kElemBf16 ? make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))
-                                                                                            : make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = p.out_elem == kElemBf16 ? make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))
+                                                                                              : make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = i * ch.step;
-    if (ch.n + j < ch.n_out) store_elem(p.out, p.out_elem, at + j, p.residual != nullptr ? v[i] + load_elem(p.residual, p.out_elem, from + j) : v[i]);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (ch.n + i * ch.step < ch.n_out) store_elem(p.out, p.out_elem, at + i * ch.step, v[i]);
 }
 
 // 32 lanes x 32 / TW consecutive columns of an accumulator
@@ -313,6 +337,12 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
 #pragma unroll 1
     for (int c = group * kChunk; c < rows; c += kI8Groups * kChunk) {
       const float f_next = chunk_factor(c + kI8Groups * kChunk);
+      Int8Residual res[kChunk / 4];
+      if (TW == 1) {
+#pragma unroll
+        for (int j = 0; j < kChunk / 4; ++j)
+          if (c + q * (kChunk / 4) + j < rows) res[j].load(p, ch, row0 + c + q * (kChunk / 4) + j);
+      }
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
         int v[kChunk];
@@ -356,7 +386,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
       for (int j = 0; j < kChunk / 4; ++j) {
         const int m = q * (kChunk / 4) + j;
         const float s = __shfl_sync(0xffffffffu, f, m);
-        if (c + m < rows) i8_store<TW>(p, ch, row0 + c + m, s, ch.sums(stage + m * 128), ch.sums(stage + ((TW - 1) * kChunk + m) * 128));
+        if (c + m < rows) i8_store<TW>(p, ch, row0 + c + m, s, ch.sums(stage + m * 128), ch.sums(stage + ((TW - 1) * kChunk + m) * 128), res[j]);
       }
       i8_group_sync(group);
       f = f_next;
@@ -414,6 +444,8 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
 #pragma unroll 2
   for (int m = first; m < rows; m += stride, ++k) {
     int4 s[TW];
+    Int8Residual res;
+    if (TW == 1) res.load(p, ch, row0 + m);
 #pragma unroll
     for (int w = 0; w < TW; ++w) {
       const int* src = stage + (w * acc_cols + m) * 128;
@@ -430,7 +462,7 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
       for (int x = 1; x < kRowsMaxSplit; ++x)
         if (x < p.splits) { s[w].x += t[x].x; s[w].y += t[x].y; s[w].z += t[x].z; s[w].w += t[x].w; }
     }
-    i8_store<TW>(p, ch, row0 + m, __shfl_sync(0xffffffffu, f, k), s[0], s[TW - 1]);
+    i8_store<TW>(p, ch, row0 + m, __shfl_sync(0xffffffffu, f, k), s[0], s[TW - 1], res);
   }
   // nobody leaves what is being read
   if (p.splits > 1) cooperative_groups::this_cluster().sync();
@@ -559,25 +591,48 @@ struct Int8Plan {
   bool clusters;
   long long counter_bytes, ws_bytes;
 };
+// The rows of a tile come from an estimate in us: a k-block of a full tile (128 x 256) 0.43 on 148 SMs, of which 0.1 are W's; an epilogue 1 and, over
+// 256 rows, 2 more; a cluster's sum 1.5.  Whole rounds waste what the last leaves idle; ranges cost about 80 k-blocks (partial sums written, awaited
+// and added).  What that chooses, and what as few tiles as possible take:
+//   700 rows against 4608 x 3584: four tiles of 176 rows 17.8 us, three of 240 20.4;  1333, 1001 x 2039: 17 of 80 rows 11.6, six of 224 14.1
+//   1000, gated 9728 x 896: eleven of 96 rows 25.6, eight of 128 30.4
+//   ranges: 1500, 3584 x 18944 123 -> 93, 8192 419 -> 401; but 2000, 3584 x 3584 49 -> 62, 4096, 8192 x 8192 193 -> 203
 static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
   Int8Plan r{};
-  const int tw = gated ? 2 : 1, most = gated ? 128 : 256;
-  r.m_tiles = (M + most - 1) / most;
-  r.mn = ((M + r.m_tiles - 1) / r.m_tiles + 15) / 16 * 16;
-  r.m_tiles = (M + r.mn - 1) / r.mn;
+  const int tw = gated ? 2 : 1, most = 256 / tw;
   r.n_tiles = (N + 128 * tw - 1) / (128 * tw);
-  r.tiles = r.m_tiles * r.n_tiles;
   r.k_blocks = (K + kI8K - 1) / kI8K;
-  r.clusters = r.tiles <= sms;
-  if (!r.clusters) {
-    // The tiles of the incomplete last round; a round more where they are so few that many CTAs would share each of them (8 tiles, 18 CTAs
-    // each: one CTA then adds 18 partial sums of 128 KB).
-    const int rest = r.tiles % sms;
-    r.cut = rest == 0 ? 0 : 7 * rest < 2 * sms ? rest + sms : rest;
-    if (r.cut > 0) {
-      r.counter_bytes = (static_cast<long long>(sms) * 4 + 1023) / 1024 * 1024;
-      r.ws_bytes = 2ll * sms * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
+  const int fewest = (M + most - 1) / most;
+  float best = 0.f;
+  for (int m_tiles = fewest; m_tiles <= fewest + 24; ++m_tiles) {
+    const int mn = ((M + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+    const long long tiles = static_cast<long long>(r.n_tiles) * ((M + mn - 1) / mn);
+    if (m_tiles > fewest && (tiles > 4 * sms || mn < 32)) break;
+    const float part = static_cast<float>(tw * mn) / 256.f, block = 0.1f * tw + 0.33f * part, epilogue = 1.f + 2.f * part;
+    float us;
+    int cut = 0;
+    if (tiles <= sms) {
+      const int splits = std::max(1, std::min({kRowsMaxSplit, static_cast<int>(sms / tiles), r.k_blocks / 2}));
+      us = static_cast<float>((r.k_blocks + splits - 1) / splits) * block + epilogue + (splits > 1 ? 1.5f : 0.f);
+    } else {
+      const int rest = static_cast<int>(tiles % sms);
+      cut = (sms - rest) * r.k_blocks > 80 * sms && rest > 0 ? rest : 0;
+      const float rounds = cut > 0 ? static_cast<float>(tiles) / static_cast<float>(sms) + 80.f / static_cast<float>(r.k_blocks)
+                                   : static_cast<float>((tiles + sms - 1) / sms);
+      us = rounds * std::max(static_cast<float>(r.k_blocks) * block, epilogue) + epilogue;
     }
+    if (m_tiles == fewest || us < 0.97f * best) {
+      best = us;
+      r.mn = mn;
+      r.m_tiles = (M + mn - 1) / mn;
+      r.cut = cut;
+    }
+  }
+  r.tiles = r.m_tiles * r.n_tiles;
+  r.clusters = r.tiles <= sms;
+  if (r.cut > 0) {
+    r.counter_bytes = (static_cast<long long>(sms) * 4 + 1023) / 1024 * 1024;
+    r.ws_bytes = 2ll * sms * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
   }
   return r;
 }
@@ -646,6 +701,7 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
   if ((ldw & 15) != 0 || ldw < K || (reinterpret_cast<uintptr_t>(w) & 15) != 0) return -4;
   if (q != nullptr && ((ldq & 15) != 0 || ldq < K || (reinterpret_cast<uintptr_t>(q) & 15) != 0)) return -4;
   if (gated != 0 && (N % 256) != 0) return -6;
+  if (static_cast<long long>((M + 15) / 16) * ((N + 127) / 128) > (1 << 30)) return -2;
   const int sms = ogb_num_sms();
   const Int8Plan plan = i8_plan(M, N, K, gated != 0, sms);
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
