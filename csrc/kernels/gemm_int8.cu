@@ -47,7 +47,7 @@ struct Int8Params {
   const float* bias;                         // or null
   const void* residual;                      // or null
   long long ldc, ldr;
-  int out_elem, vec;                         // vec: results and residuals in pieces of four
+  int vec;                                   // results and residuals in pieces of four
   int M, N, mn;                              // mn: rows of a tile, a multiple of 16
   int n_tiles, m_tiles, tiles, k_blocks, stages;
   int splits;                                // CTAs (a cluster) per tile; 0: whole tiles and ranges
@@ -184,68 +184,95 @@ struct Int8Channels {
   }
 };
 // A lane's four residuals of a row, fetched ahead of the sums they are added to.
+template <int OUT>
 struct Int8Residual {
-  uint4 raw;
+  uint32_t raw[OUT == kElemF32 ? 4 : 2];
   template <int TW>
   OGB_DEVICE void load(const Int8Params& p, const Int8Channels<TW>& ch, int m) {
-    raw = make_uint4(0, 0, 0, 0);
-    if (p.residual == nullptr) return;
     const size_t from = static_cast<size_t>(m) * p.ldr + ch.n;
     if (p.vec != 0 && ch.n + 4 <= ch.n_out) {
-      if (p.out_elem == kElemF32) {
-        raw = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + from);
+      if constexpr (OUT == kElemF32) {
+        const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const float*>(p.residual) + from);
+        raw[0] = r.x; raw[1] = r.y; raw[2] = r.z; raw[3] = r.w;
       } else {
         const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + from);
-        raw.x = r.x;
-        raw.y = r.y;
+        raw[0] = r.x; raw[1] = r.y;
       }
       return;
     }
-    float v[4];
+    uint32_t v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = ch.n + i * ch.step < ch.n_out ? load_elem(p.residual, p.out_elem, from + i * ch.step) : 0.f;
-    // as the type's own bits again: what add() reads
-    if (p.out_elem == kElemF32) raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    else if (p.out_elem == kElemBf16) raw = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), 0, 0);
-    else raw = make_uint4(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), 0, 0);
-  }
-  OGB_DEVICE void add(const Int8Params& p, float (&v)[4]) const {
-    if (p.out_elem == kElemF32) {
-      v[0] += __uint_as_float(raw.x); v[1] += __uint_as_float(raw.y); v[2] += __uint_as_float(raw.z); v[3] += __uint_as_float(raw.w);
-      return;
+    for (int i = 0; i < 4; ++i) {
+      const bool in = ch.n + i * ch.step < ch.n_out;
+      if constexpr (OUT == kElemF32) v[i] = in ? static_cast<const uint32_t*>(p.residual)[from + i * ch.step] : 0;
+      else v[i] = in ? static_cast<const uint16_t*>(p.residual)[from + i * ch.step] : 0;
     }
-    const float2 lo = p.out_elem == kElemBf16 ? unpack_bf16(raw.x) : __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
-    const float2 hi = p.out_elem == kElemBf16 ? unpack_bf16(raw.y) : __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
-    v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+    if constexpr (OUT == kElemF32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = v[i];
+    } else {
+      raw[0] = v[0] | v[1] << 16;
+      raw[1] = v[2] | v[3] << 16;
+    }
+  }
+  OGB_DEVICE void add(float (&v)[4]) const {
+    if constexpr (OUT == kElemF32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(raw[i]);
+    } else {
+      const float2 lo = OUT == kElemBf16 ? unpack_bf16(raw[0]) : __half22float2(*reinterpret_cast<const __half2*>(&raw[0]));
+      const float2 hi = OUT == kElemBf16 ? unpack_bf16(raw[1]) : __half22float2(*reinterpret_cast<const __half2*>(&raw[1]));
+      v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+    }
   }
 };
-// Sums of row m (and of the up half) -> the stored result.
-template <int TW>
-OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m, float s, const int4& a, const int4& u, const Int8Residual& r) {
-  if (ch.n >= ch.n_out) return;                               // the others are further on
-  const int raw[4] = {a.x, a.y, a.z, a.w}, up[4] = {u.x, u.y, u.z, u.w};
-  float v[4];
+// Sums of R rows (and of their up halves) -> the stored results; row j is m0 + j * step, there if below `end`.  All rows are computed before the first is
+// stored: one after the other each took a chain of 500 cycles.
+template <int TW, int OUT, int R>
+OGB_DEVICE void i8_store(const Int8Params& p, const Int8Channels<TW>& ch, int m0, int step, int end, const float (&s)[R], const int4 (&a)[R],
+                         const int4 (&u)[R], const Int8Residual<OUT> (&res)[R]) {
+  float v[R][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = fmaf(static_cast<float>(raw[i]) * s, ch.c[0][i], ch.b[0][i]);
-    if constexpr (TW == 2) {
-      const float w = fmaf(static_cast<float>(up[i]) * s, ch.c[TW - 1][i], ch.b[TW - 1][i]);
-      v[i] = __fdividef(v[i], 1.f + __expf(-v[i])) * w;
+  for (int j = 0; j < R; ++j) {
+    const int raw[4] = {a[j].x, a[j].y, a[j].z, a[j].w}, up[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[j][i] = fmaf(static_cast<float>(raw[i]) * s[j], ch.c[0][i], ch.b[0][i]);
+      if constexpr (TW == 2) {
+        const float w = fmaf(static_cast<float>(up[i]) * s[j], ch.c[TW - 1][i], ch.b[TW - 1][i]);
+        v[j][i] = __fdividef(v[j][i], 1.f + __expf(-v[j][i])) * w;
+      }
     }
   }
-  if (TW == 1 && p.residual != nullptr) r.add(p, v);
-  const size_t at = static_cast<size_t>(m) * p.ldc + ch.n;
+  if (TW == 1 && p.residual != nullptr) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) res[j].add(v[j]);
+  }
   if (p.vec != 0 && ch.n + 4 <= ch.n_out) {
-    if (p.out_elem == kElemF32)
-      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-    else
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = p.out_elem == kElemBf16 ? make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))
-                                                                                              : make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int m = m0 + j * step;
+      const size_t at = static_cast<size_t>(m) * p.ldc + ch.n;
+      if (m < end) {
+        if constexpr (OUT == kElemF32)
+          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+        else
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+              OUT == kElemBf16 ? make_uint2(pack_bf16(v[j][0], v[j][1]), pack_bf16(v[j][2], v[j][3])) : make_uint2(pack_f16(v[j][0], v[j][1]), pack_f16(v[j][2], v[j][3]));
+      }
+    }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (ch.n + i * ch.step < ch.n_out) store_elem(p.out, p.out_elem, at + i * ch.step, v[i]);
+  for (int j = 0; j < R; ++j) {
+    const int m = m0 + j * step;
+    const size_t at = static_cast<size_t>(m) * p.ldc + ch.n;
+    if (m < end) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ch.n + i * ch.step < ch.n_out) store_elem(p.out, OUT, at + i * ch.step, v[j][i]);
+    }
+  }
 }
 
 // 32 lanes x 32 / TW consecutive columns of an accumulator
@@ -268,7 +295,7 @@ OGB_DEVICE void i8_group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r
 
 // The epilogue warps, where whole tiles and ranges are computed.  Warp index mod 4: the quarter of TMEM's lanes, 32 channels of a tile; each of the
 // two groups takes every other chunk of rows.
-template <int TW>
+template <int TW, int OUT>
 OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars, int* staging) {
   constexpr int kChunk = kI8Chunk<TW>;
   const int warp = (threadIdx.x >> 5) - 2, q = (threadIdx.x >> 5) & 3, group = warp >> 2, lane = threadIdx.x & 31;
@@ -288,6 +315,20 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     int nt, mt;
     i8_tile(p, tile, nt, mt);
     const int row0 = mt * p.mn, rows = min(p.mn, p.M - row0);
+    // what the tile's epilogue needs besides its sums, while they are under way
+    const Int8Channels<TW> ch(p, nt);
+    // the factors of a chunk's rows, a lane each
+    auto chunk_factor = [&](int c) { return lane < kChunk && c + lane < rows ? factor[row0 + c + lane] : 0.f; };
+    Int8Residual<OUT> res[kChunk / 4];
+    auto chunk_residual = [&](int c) {
+      if (TW == 1 && p.residual != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kChunk / 4; ++j)
+          if (c + q * (kChunk / 4) + j < rows) res[j].load(p, ch, row0 + c + q * (kChunk / 4) + j);
+      }
+    };
+    float f = chunk_factor(group * kChunk);
+    chunk_residual(group * kChunk);
     // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out the warps go on
     // to arrive on the counters of their shared tiles.
     if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[buf], buf_phase))) {
@@ -330,19 +371,9 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     } else if (!ok) {
       continue;
     }
-    const Int8Channels<TW> ch(p, nt);
-    // the factors of a chunk's rows, a lane each
-    auto chunk_factor = [&](int c) { return lane < kChunk && c + lane < rows ? factor[row0 + c + lane] : 0.f; };
-    float f = chunk_factor(group * kChunk);
 #pragma unroll 1
     for (int c = group * kChunk; c < rows; c += kI8Groups * kChunk) {
       const float f_next = chunk_factor(c + kI8Groups * kChunk);
-      Int8Residual res[kChunk / 4];
-      if (TW == 1) {
-#pragma unroll
-        for (int j = 0; j < kChunk / 4; ++j)
-          if (c + q * (kChunk / 4) + j < rows) res[j].load(p, ch, row0 + c + q * (kChunk / 4) + j);
-      }
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
         int v[kChunk];
@@ -382,12 +413,17 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
         for (int j = 0; j < kChunk; ++j) stage[(w * kChunk + j) * 128 + q * 32 + lane] = v[j];
       }
       i8_group_sync(group);
+      float s[kChunk / 4];
+      int4 a[kChunk / 4], u[kChunk / 4];
 #pragma unroll
       for (int j = 0; j < kChunk / 4; ++j) {
         const int m = q * (kChunk / 4) + j;
-        const float s = __shfl_sync(0xffffffffu, f, m);
-        if (c + m < rows) i8_store<TW>(p, ch, row0 + c + m, s, ch.sums(stage + m * 128), ch.sums(stage + ((TW - 1) * kChunk + m) * 128), res[j]);
+        s[j] = __shfl_sync(0xffffffffu, f, m);
+        a[j] = ch.sums(stage + m * 128);
+        u[j] = TW == 2 ? ch.sums(stage + ((TW - 1) * kChunk + m) * 128) : a[j];
       }
+      i8_store<TW, OUT>(p, ch, row0 + c + q * (kChunk / 4), 1, row0 + rows, s, a, u, res);
+      chunk_residual(c + kI8Groups * kChunk);
       i8_group_sync(group);
       f = f_next;
     }
@@ -400,7 +436,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
 }
 
 // All threads of a CTA, after their parts of the main loop: the epilogue of a tile that a cluster shares.  smem: the ring, free by then.
-template <int TW>
+template <int TW, int OUT>
 OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int acc_cols, RowsBars* bars, uint8_t* smem, int ring_bytes) {
   constexpr int kChunk = kI8Chunk<TW>;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -440,29 +476,35 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
   }
   if (p.splits > 1) cooperative_groups::this_cluster().sync();
   else __syncthreads();
-  int k = 0;
-#pragma unroll 2
-  for (int m = first; m < rows; m += stride, ++k) {
-    int4 s[TW];
-    Int8Residual res;
-    if (TW == 1) res.load(p, ch, row0 + m);
+  constexpr int kRows = 4 / TW;                     // at a time
+  for (int m0 = first, k = 0; m0 < rows; m0 += stride * kRows, k += kRows) {
+    float s[kRows];
+    int4 sum[TW][kRows];
+    Int8Residual<OUT> res[kRows];
 #pragma unroll
-    for (int w = 0; w < TW; ++w) {
-      const int* src = stage + (w * acc_cols + m) * 128;
-      if (p.splits == 1) {
-        s[w] = ch.sums(src);
-        continue;
-      }
-      int4 t[kRowsMaxSplit];
-#pragma unroll
-      for (int x = 0; x < kRowsMaxSplit; ++x)
-        if (x < p.splits) t[x] = ch.sums(cooperative_groups::this_cluster().map_shared_rank(src, x));
-      s[w] = t[0];
-#pragma unroll
-      for (int x = 1; x < kRowsMaxSplit; ++x)
-        if (x < p.splits) { s[w].x += t[x].x; s[w].y += t[x].y; s[w].z += t[x].z; s[w].w += t[x].w; }
+    for (int j = 0; j < kRows; ++j) {
+      s[j] = __shfl_sync(0xffffffffu, f, (k + j) & 31);
+      if (TW == 1 && p.residual != nullptr && m0 + stride * j < rows) res[j].load(p, ch, row0 + m0 + stride * j);
     }
-    i8_store<TW>(p, ch, row0 + m, __shfl_sync(0xffffffffu, f, k), s[0], s[TW - 1], res);
+#pragma unroll
+    for (int w = 0; w < TW; ++w)
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int* src = stage + (w * acc_cols + min(m0 + stride * j, rows - 1)) * 128;
+        if (p.splits == 1) {
+          sum[w][j] = ch.sums(src);
+          continue;
+        }
+        int4 t[kRowsMaxSplit];
+#pragma unroll
+        for (int x = 0; x < kRowsMaxSplit; ++x)
+          if (x < p.splits) t[x] = ch.sums(cooperative_groups::this_cluster().map_shared_rank(src, x));
+        sum[w][j] = t[0];
+#pragma unroll
+        for (int x = 1; x < kRowsMaxSplit; ++x)
+          if (x < p.splits) { sum[w][j].x += t[x].x; sum[w][j].y += t[x].y; sum[w][j].z += t[x].z; sum[w][j].w += t[x].w; }
+      }
+    i8_store<TW, OUT>(p, ch, row0 + m0, stride, row0 + rows, s, sum[0], sum[TW - 1], res);
   }
   // nobody leaves what is being read
   if (p.splits > 1) cooperative_groups::this_cluster().sync();
@@ -501,7 +543,7 @@ OGB_DEVICE bool i8_issue_mma(const Int8Params& p, uint8_t* smem, int stage_bytes
   return true;
 }
 
-template <int TW>
+template <int TW, int OUT>
 __global__ void __launch_bounds__(kI8Threads, 1)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q, const Int8Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -576,9 +618,9 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     }
     __syncwarp();
   } else if (p.splits == 0) {
-    i8_epilogue<TW>(p, tmem_base, bufs, acc_cols, bars, staging);
+    i8_epilogue<TW, OUT>(p, tmem_base, bufs, acc_cols, bars, staging);
   }
-  if (p.splits > 0) i8_finish_cluster<TW>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
+  if (p.splits > 0) i8_finish_cluster<TW, OUT>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
   rows_teardown(bars, tmem_base, tmem_cols);
 }
 
@@ -637,9 +679,9 @@ static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
   return r;
 }
 
-template <int TW>
+template <int TW, int OUT>
 static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long long ldq, const void* w, long long ldw, int K, bool early, cudaStream_t stream) {
-  auto kernel = gemm_int8_kernel<TW>;
+  auto kernel = gemm_int8_kernel<TW, OUT>;
   static OncePerDevice allowed;
   int rc = allow_smem(allowed, kernel, kRowsSmemMax);
   if (rc != 0) return rc;
@@ -727,11 +769,18 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
     early = false;
   }
   p.out = out; p.factor = factor; p.channel = channel; p.bias = bias; p.residual = residual;
-  p.ldc = ldc; p.ldr = ldr; p.out_elem = out_elem;
+  p.ldc = ldc; p.ldr = ldr;
   const int piece = 4 * elem_bytes(out_elem);
   p.vec = (reinterpret_cast<uintptr_t>(out) % piece == 0 && ldc % 4 == 0 &&
            (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) % piece == 0 && ldr % 4 == 0))) ? 1 : 0;
   p.M = M; p.N = N; p.mn = plan.mn; p.n_tiles = plan.n_tiles; p.m_tiles = plan.m_tiles; p.tiles = plan.tiles; p.k_blocks = plan.k_blocks;
   p.cut = plan.cut; p.range = plan.cut * plan.k_blocks / sms; p.longer = plan.cut * plan.k_blocks % sms; p.status = status;
-  return gated != 0 ? launch_int8<2>(plan, p, q, ldq, w, ldw, K, early, stream) : launch_int8<1>(plan, p, q, ldq, w, ldw, K, early, stream);
+  if (gated != 0) {
+    if (out_elem == kElemF32) return launch_int8<2, kElemF32>(plan, p, q, ldq, w, ldw, K, early, stream);
+    if (out_elem == kElemBf16) return launch_int8<2, kElemBf16>(plan, p, q, ldq, w, ldw, K, early, stream);
+    return launch_int8<2, kElemF16>(plan, p, q, ldq, w, ldw, K, early, stream);
+  }
+  if (out_elem == kElemF32) return launch_int8<1, kElemF32>(plan, p, q, ldq, w, ldw, K, early, stream);
+  if (out_elem == kElemBf16) return launch_int8<1, kElemBf16>(plan, p, q, ldq, w, ldw, K, early, stream);
+  return launch_int8<1, kElemF16>(plan, p, q, ldq, w, ldw, K, early, stream);
 }
