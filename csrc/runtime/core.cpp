@@ -314,6 +314,7 @@ void Core::publish_full_pages(Sequence& s) {
 
 void Core::try_prefix_attach(Sequence& s) {
   if (!cfg_.enable_prefix_cache || !s.pages.empty()) return;
+  if (s.forced && !s.wanted.empty()) return;               // its logits rows come from computing the positions, cached or not
   // never serve the whole prompt from cache: the last token must run to produce logits
   const int max_full = (static_cast<int>(s.tokens.size()) - 1) / kPageTokens;
   uint64_t h = 0;
