@@ -11,6 +11,7 @@ from __future__ import annotations
 import argparse
 import copy
 import json
+import math
 import os
 import sys
 import time
@@ -44,6 +45,7 @@ def _add_engine(p):
                         "(any decoder architecture, `generate` only, one sequence)")
     p.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "fp8_e4m3fn", "fp8_e5m2", "int8"])
     p.add_argument("--compute-dtype", default="bf16", choices=["bf16", "f32"], help="f32: weights, activations and cache in true 32-bit (checkpoint architectures that have it)")
+    p.add_argument("--weight-dtype", default="bf16", choices=["bf16", "int8"], help="int8: dense layers in 8 bits with a factor per channel, activations quantised a token at a time")
     p.add_argument("--max-batch", type=int, default=32)
     p.add_argument("--vram-limit", default="0.85", help="0.85 (fraction of the device the engine may fill), auto, or a size such as 8GiB for weights + activations + KV")
     p.add_argument("--context-cache", action="store_true", help="keep the lowered weight layout beside the model (ogb_context/) and reuse it on the next load")
@@ -124,6 +126,10 @@ def _load(args):
         extra["context_cache"] = True
     if getattr(args, "compute_dtype", "bf16") != "bf16":
         extra["compute_dtype"] = args.compute_dtype
+    if getattr(args, "weight_dtype", "bf16") != "bf16":
+        extra["weight_dtype"] = args.weight_dtype
+    if getattr(args, "logit_rows", 0) > 0:
+        extra["max_logit_rows"] = args.logit_rows
     if getattr(args, "weight_offload_layers", 0) > 0:
         extra["weight_offload_layers"] = args.weight_offload_layers
     eng = Engine.from_dir(args.model, device=dev, max_seqs=args.max_batch, kv_dtype={"fp8_e4m3fn": "fp8", "int8": "int8", "fp8_e5m2": "fp8_e5m2"}.get(args.kv_cache_dtype, "bf16"),
@@ -560,6 +566,28 @@ def _save_png(path: str, chw) -> None:
         f.write(encode_png(chw))
 
 
+def cmd_score(args, profiler):
+    """Log probabilities of given texts under the model, a JSON line each, and the perplexity of all of them together."""
+    eng = _load(args)
+    if eng.tokenizer is None and not args.ids:
+        print("score: this model directory has no tokenizer.json; give token ids, with --ids", file=sys.stderr)
+        return 2
+    lines = args.text or [line.rstrip("\n") for line in sys.stdin]
+    try:
+        texts = [[int(t) for t in line.replace(",", " ").split()] for line in lines] if args.ids else lines
+        docs = eng.score([t for t in texts if len(t)], top=args.top)
+    except ValueError as e:
+        print(f"score: {e}", file=sys.stderr)
+        return 2
+    total, count = 0.0, 0
+    for doc in docs:
+        print(json.dumps(doc))
+        total, count = total + sum(doc["logprobs"]), count + len(doc["logprobs"])
+    if count:
+        print(f"{len(docs)} texts, {count} tokens scored, perplexity {math.exp(-total / count):.4f}", file=sys.stderr)
+    return 0
+
+
 def cmd_show(args, profiler):
     from . import package as pkg
     from .package.onnx_text import load_any
@@ -965,6 +993,14 @@ def main(argv=None):
     _add_engine(r)
     r.add_argument("--multimodal-package", default="",
                    help="workflow package with a typed image or audio input: /image and /audio attachments are answered by it")
+    sc = sub.add_parser("score", help="log probabilities and perplexity of given texts")
+    sc.add_argument("model")
+    sc.add_argument("--text", action="append", default=[], help="a text to score (repeatable; without any, a line each on standard input)")
+    sc.add_argument("--ids", action="store_true", help="texts are token ids (commas or spaces)")
+    sc.add_argument("--top", type=int, default=0, help="list the likeliest tokens in each place too (at most 32)")
+    sc.add_argument("--logit-rows", type=int, default=512, help="tokens scored in one step")
+    sc.add_argument("--max-context", type=int, default=0)
+    _add_engine(sc)
     s = sub.add_parser("serve")
     s.add_argument("model", nargs="?", default="", help="model directory (or use --models-dir)")
     s.add_argument("--models-dir", default="", help="serve every model directory below this one; requests pick one by name")
@@ -1067,7 +1103,7 @@ def main(argv=None):
         print(f"onnx-genai-b200 {__version__}")
         return 0
     profiler = Profiler(args.profile, args.profile_json, args.profile_trace, gpu=getattr(args, "profile_gpu", False))
-    return {"generate": cmd_generate, "run": cmd_run, "serve": cmd_serve, "show": cmd_show, "validate": cmd_validate, "list": cmd_list,
+    return {"generate": cmd_generate, "run": cmd_run, "score": cmd_score, "serve": cmd_serve, "show": cmd_show, "validate": cmd_validate, "list": cmd_list,
             "export": cmd_export, "transcribe": cmd_transcribe}[args.cmd](args, profiler)
 
 

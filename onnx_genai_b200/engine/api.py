@@ -277,7 +277,15 @@ class Engine:
             cproc = cons.ConstraintProcessor(cons.make_constraint(opt.constraint), self.token_texts(), stop_ids)
         chain = procs.build_processor_chain(eff, len(ids), rng, extra=processors, constraint=cproc)
         plan = procs.device_sampling_plan(chain, eff, sampler is not None)
+        # Greedy requests whose only wish beyond the device's own path are log probabilities get them there (ops.token_logprobs); a row of
+        # logits does not cross to the host.
+        on_device = (opt.logprobs and self.llm.device.type == "cuda" and self.llm.tp == 1 and self.llm.pp == 1 and not opt.speculative
+                     and procs.device_sampling_plan(chain, GenerateOptions(**{**eff.__dict__, "logprobs": 0}), sampler is not None) == "greedy")
+        if on_device:
+            plan = "greedy"
         state = {"ids": list(int(i) for i in ids), "chain": chain, "logprobs": [], "plan": plan, "constraint": cproc}
+        if on_device:
+            self.llm.device_logprobs[sid & 0x7FFFFFFF] = (opt.logprobs, state["logprobs"])
         if plan == "host":
             smp = sampler or (procs.GreedySampler() if greedy else procs.CategoricalSampler())
 
@@ -304,6 +312,21 @@ class Engine:
             else:
                 self.llm.proposers[sid] = NgramProposer()
         return sid, state
+
+    def score(self, texts, top: int = 0) -> list:
+        """How likely the model finds each text (a string or token ids): ``{"token_ids", "logprobs", "ranks", "entropies", "perplexity"}`` with one entry a
+        token from the second on, and with ``top`` the likeliest tokens and their log probabilities in each place (``"top"``).  Runs the
+        engine by itself: no request may be in flight."""
+        ids = [self.tokenize(t) if isinstance(t, str) else [int(i) for i in t] for t in texts]
+        out = []
+        for tokens, r in zip(ids, self.llm.score(ids, top=top, entropy=True)):
+            n = len(tokens) - 1
+            doc = {"token_ids": tokens, "logprobs": r.logprob.tolist(), "ranks": r.rank.tolist(), "entropies": r.entropy.tolist(),
+                   "perplexity": float(np.exp(-float(r.logprob.double().mean()))) if n else None}
+            if top:
+                doc["top"] = [list(zip(i, v)) for i, v in zip(r.top_ids.tolist(), r.top_logprobs.tolist())]
+            out.append(doc)
+        return out
 
     def token_texts(self) -> list:
         """Decoded text of every vocabulary entry ('' for special tokens and incomplete byte sequences);
@@ -358,6 +381,7 @@ class Engine:
             except Exception:          # offload is an optimisation: a full disk must not fail the request
                 pass
         self.llm.host_samplers.pop(sid & 0x7FFFFFFF, None)
+        self.llm.device_logprobs.pop(sid & 0x7FFFFFFF, None)
         prop = self.llm.proposers.pop(sid, None)
         if prop is not None and hasattr(prop, "close"):
             prop.close()

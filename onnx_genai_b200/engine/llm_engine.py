@@ -28,7 +28,7 @@ import torch
 
 from .. import ops
 from ..models.config import DecoderConfig
-from ..models.decoder import DecoderWeights, KVCache, StepInputs
+from ..models.decoder import DecoderWeights, KVCache, StepInputs, quantize_int8
 from ..models.registry import family_of
 from ..models.state import StateCache
 from ..parallel.sharding import shard_heads
@@ -56,6 +56,8 @@ class EngineConfig:
     release_window_pages: bool = True  # sliding-window models: give back the KV pages no later query can see (sinks are kept)
     kv_dtype: str = "bf16"
     compute_dtype: str = "bf16"        # "f32": weights, activations and pages in true 32-bit (families that have it)
+    weight_dtype: str = "bf16"         # "int8": the layers' matrices in 8 bits with a factor per channel, activations quantised a token at a time
+                                       # (dense decoders on one GPU; the weights handed in are converted in place)
     max_logit_rows: int = 0            # logits rows a step may produce (0: one per sequence and draft)
     decode_splits: int = 0             # 0: pick from batch shape
     sync_sampled_tokens: bool = True   # TP: broadcast rank 0's tokens so replicas cannot diverge
@@ -120,6 +122,12 @@ class LLMEngine:
         if weights is None:
             dtype = torch.bfloat16 if is_cuda and cfg.compute_dtype == "bf16" else torch.float32
             weights = fam.random_weights(m, self.device, tp, shard_rank, cfg.seed, dtype)
+        if cfg.weight_dtype not in ("bf16", "int8"):
+            raise ValueError(f"weight_dtype {cfg.weight_dtype!r} is not supported; use bf16 (weights as they come) or int8")
+        if cfg.weight_dtype == "int8":
+            if not isinstance(weights, DecoderWeights) or tp > 1 or self.pp > 1 or cfg.weight_offload_layers or cfg.compute_dtype != "bf16":
+                raise ValueError("8-bit weights are made for dense bf16 decoders on one GPU, without weight offload")
+            quantize_int8(weights)
         self.weights = weights
         max_pages_per_seq = (cfg.max_seq_len + ops.PAGE - 1) // ops.PAGE
         hs = shard_heads(m.num_heads, m.num_kv_heads, tp, shard_rank)
@@ -260,6 +268,9 @@ class LLMEngine:
             self.memory.lease("weights", "host", self.model.paged_weight_bytes, f"{cfg.weight_offload_layers} paged layer(s)")
             slots = sum(s.numel() for s in self.model.weight_slots)
             self.weights_lease.resize(max(0, self.weights_lease.nbytes - self.model.paged_weight_bytes + slots))   # two slots stay on the device
+        self.logit_row_limit = max_rows
+        self.scoring: dict = {}           # forced sequence of score() -> (next token of every position, top, entropy, results)
+        self.device_logprobs: dict = {}   # seq id -> (top, list): the log probability of each of its tokens and the likeliest, as it is sampled
         self.host_samplers: dict = {}     # seq id -> fn(logits_row fp32 numpy, uniform) -> token id
         self.forced: set = set()          # sequences whose tokens come from the caller (open_forced)
         self.proposers: dict = {}         # seq id -> SpeculativeProposer
@@ -315,18 +326,73 @@ class LLMEngine:
         """Tokens of a forced sequence that no step has computed yet."""
         return self.core.seq_len(sid) - self.core.seq_computed(sid)
 
+    def score(self, prompts, top: int = 0, entropy: bool = False) -> list:
+        """Log probabilities of the tokens of each prompt (token ids) given those before them: one ``ops.TokenLogprobs`` of CPU tensors per prompt,
+        its row k for token k + 1 (nothing says how likely the first one is).  Rows never leave the device as logits.  Runs the engine by
+        itself, a step's worth of rows at a time (``max_logit_rows``): no request may be in flight."""
+        if self.tp > 1 or self.pp > 1:
+            raise ValueError("score() runs on one GPU")
+        if self.has_work or self.stats or self.forced:
+            raise RuntimeError("score() drives the engine by itself: finish the requests in flight first")
+        rows = self.logit_row_limit
+        results = []
+        for tokens in prompts:
+            tokens = [int(t) for t in tokens]
+            if not tokens or min(tokens) < 0 or max(tokens) >= self.cfg.model.vocab:
+                raise ValueError(f"a prompt to score is one or more token ids in [0, {self.cfg.model.vocab})")
+            sid, done, parts = None, 0, []
+            try:
+                while done < len(tokens):
+                    piece = tokens[done:done + rows]
+                    want = range(min(len(piece), len(tokens) - 1 - done))
+                    if sid is None:
+                        sid = self.open_forced(piece, want)
+                        self.scoring[sid] = (torch.tensor(tokens[1:] + [-1], dtype=torch.int32, device=self.device), int(top), bool(entropy), parts)
+                    else:
+                        self.extend_forced(sid, piece, want)
+                    while self.forced_pending(sid) > 0:
+                        if self.step().num_tokens == 0:
+                            raise RuntimeError("the scheduler could not run the prompt: it needs more KV pages than there are")
+                    done += len(piece)
+            finally:
+                if sid is not None:
+                    self.scoring.pop(sid, None)
+                    self.close_forced(sid)
+            empty = ops.token_logprobs(torch.zeros(0, self.cfg.model.vocab), torch.zeros(0, dtype=torch.int32), top, entropy)
+            results.append(ops.TokenLogprobs(*(None if e is None else torch.cat([e] + [p[i].cpu() for p in parts]) for i, e in enumerate(empty))))
+        return results
+
     def _collect_forced(self, out: "StepOutput", logits, r: int) -> int:
         """Copies the rows of forced sequences out of the step's logits; returns how many of the r rows they were."""
         L, pn = self.L, self.plan_np
         seqs = pn[L.logit_seq:L.logit_seq + r]
         by_key = {sid & 0x7FFFFFFF: sid for sid in self.forced}
         rows = [i for i in range(r) if int(seqs[i]) in by_key]
-        if rows:
+        if self.scoring and rows:           # score(): the one sequence there is, and its rows are consecutive
+            tokens, top, entropy, parts = self.scoring[by_key[int(seqs[rows[0]])]]
+            pos = int(pn[L.positions + int(pn[L.logit_rows + rows[0]])])
+            lo, hi = rows[0], rows[-1] + 1
+            parts.append(ops.token_logprobs(logits[lo:hi], tokens[pos:pos + hi - lo], top=top, entropy=entropy))
+        elif rows:
             block = logits[rows].float()
             for j, i in enumerate(rows):
                 pos = int(pn[L.positions + int(pn[L.logit_rows + i])])
                 out.forced_logits.setdefault(by_key[int(seqs[i])], []).append((pos, block[j]))
         return len(rows)
+
+    def _collect_logprobs(self, logits, r: int) -> None:
+        """Log probabilities of the tokens just sampled, for the requests that ask: only these and the likeliest cross to the host."""
+        seqs = self.plan_np[self.L.logit_seq:self.L.logit_seq + r]
+        asked = {i: self.device_logprobs[int(seqs[i])] for i in range(r) if int(seqs[i]) in self.device_logprobs}
+        if not asked:
+            return
+        lo, hi = min(asked), max(asked) + 1
+        tokens = self.sampled_dev[lo:hi] if self.device.type == "cuda" else self.sampled_host[lo:hi]
+        got = ops.token_logprobs(logits[lo:hi], tokens, top=max(top for top, _ in asked.values()))
+        lp, ids, lps = got.logprob.cpu(), got.top_ids.cpu(), got.top_logprobs.cpu()
+        self.d2h_bytes += 4 * (lp.numel() + 2 * ids.numel())
+        for i, (top, sink) in asked.items():
+            sink.append((float(lp[i - lo]), [(int(t), float(v)) for t, v in zip(ids[i - lo, :top], lps[i - lo, :top])]))
 
     @property
     def has_work(self) -> bool:
@@ -635,7 +701,7 @@ class LLMEngine:
         ids (4 bytes per row) replaces the broadcast that kept replicas in step.  Steps whose logits are needed on
         the host (custom samplers, log-probabilities, embeddings, speculative verification) keep all rows."""
         return (self.tp > 1 and self.cfg.shard_sampling and r >= self.tp
-                and not self.host_samplers and not self.hidden_taps and not self.forced and self.cfg.max_draft_tokens == 0)
+                and not self.host_samplers and not self.device_logprobs and not self.hidden_taps and not self.forced and self.cfg.max_draft_tokens == 0)
 
     def forward_and_sample_sharded(self, si, r: int, greedy: bool) -> None:
         """Run the step with this rank's share of the sampling rows; leaves all r token ids in sampled_dev[:r]."""
@@ -804,6 +870,8 @@ class LLMEngine:
                 key = int(seq_of_row[row])
                 if key in self.hidden_taps and self.hidden_taps[key] is None:
                     self.hidden_taps[key] = self.model.h_last[row].float().cpu().numpy().copy()
+        if self.device_logprobs and r > 0:
+            self._collect_logprobs(logits, r)
         if self.host_samplers and r > 0:
             # rows whose request cannot use the device sampler: logits cross to the host, the request's
             # processor chain and sampler pick the token, and the device's choice for that row is replaced

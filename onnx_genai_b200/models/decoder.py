@@ -40,6 +40,7 @@ class LayerWeights:
     expert_gate_up: torch.Tensor | None = None  # [E_local, 2*I, H] packed per expert
     expert_down: torch.Tensor | None = None     # [E_local, H, I]
     quant: dict = field(default_factory=dict)   # int4 tensors keyed by projection name
+    int8: dict = field(default_factory=dict)    # 8-bit weights (ops.int8) keyed by projection name: qkv, o, gate_up, down; qkv_b: bias in fp32
 
 
 @dataclass
@@ -68,6 +69,27 @@ def pad_mlp(gate, up, down, multiple: int = 64):
     z = torch.zeros(pad, gate.shape[1], dtype=gate.dtype, device=gate.device)
     zd = torch.zeros(down.shape[0], pad, dtype=down.dtype, device=down.device)
     return torch.cat([gate, z], 0), torch.cat([up, z], 0), torch.cat([down, zd], 1)
+
+
+def quantize_int8(weights: DecoderWeights) -> DecoderWeights:
+    """Turns the layers' matrices into 8-bit weights with a factor per channel, in place and one layer at a time; their products quantise
+    activations a token at a time (ops.int8).  Embeddings, norms and the LM head stay as they are.  For dense layers on one GPU."""
+    from ..ops import int8
+
+    half = weights.swiglu_half
+    for i, l in enumerate(weights.layers):
+        if l.int8:
+            continue
+        if l.quant or l.router_w is not None or l.gate_up_w is None:
+            raise ValueError(f"layer {i} has {'int4' if l.quant else 'expert'} weights: 8-bit weights are made of dense ones")
+        w = l.gate_up_w
+        blocks = w.view(-1, 2, half, w.shape[1])
+        gate_up = int8.quantize_gate_up(blocks[:, 0].reshape(-1, w.shape[1]), blocks[:, 1].reshape(-1, w.shape[1]))
+        down = torch.nn.functional.pad(l.down_w, (0, gate_up.q.shape[0] // 2 - l.down_w.shape[1]))
+        l.int8 = {"qkv": int8.quantize_weight(l.qkv_w), "o": int8.quantize_weight(l.o_w), "gate_up": gate_up, "down": int8.quantize_weight(down),
+                  "qkv_b": None if l.qkv_b is None else l.qkv_b.float().contiguous()}
+        l.qkv_w = l.qkv_b = l.o_w = l.gate_up_w = l.down_w = None
+    return weights
 
 
 def random_weights(cfg: DecoderConfig, device, tp: int = 1, rank: int = 0, seed: int = 0, std: float = 0.02,
@@ -316,8 +338,13 @@ class DecoderModel:
         self.qkv = z(max_tokens, (self.hq + 2 * self.hkv) * self.d)
         self.attn = z(max_tokens, self.hq * self.d)
         inter_local = (weights.layers[0].gate_up_w.shape[0] // 2) if weights.layers[0].gate_up_w is not None else 0
+        self.int8 = bool(weights.layers[0].int8)
+        if self.int8:
+            if tp != 1:
+                raise ValueError("8-bit weights run on one GPU")
+            inter_local = weights.layers[0].int8["down"].q.shape[1]
         self.act = z(max_tokens, max(inter_local, 8))
-        self.partial = z(max_tokens, hid) if tp > 1 else None
+        self.partial = z(max_tokens, hid) if tp > 1 or self.int8 else None
         if any(l.quant for l in weights.layers):     # MatMulNBits layers: build the int4 projections
             from ..ops.quant import QuantLinear
 
@@ -352,7 +379,7 @@ class DecoderModel:
 
     def bind_native(self, kv: "KVCache", max_pages_per_seq: int) -> bool:
         """Create the C++ step executor over this model's buffers; returns False when the
-        configuration needs the Python-driven path (TP > 1, MoE, int4 weights, fp8 pages, CPU)."""
+        configuration needs the Python-driven path (TP > 1, MoE, int4 or 8-bit weights, fp8 pages, CPU)."""
         import ctypes
 
         from ..ops import _native
@@ -573,6 +600,9 @@ class DecoderModel:
                 lw.quant["gate_up"].fused(x, gu, norm_weight=lw.ln2, eps=cfg.rms_eps)
                 lw.quant["down"].fused(gu, x, silu_mul=True, residual=x)
                 continue
+            if lw.int8:
+                pending = self._int8_layer(si, kv, li, lw, x, pending)
+                continue
             self._norm(x, lw.ln1, pending, h)
             if tapping and li in self.taps:       # the norm has just folded the previous layer's output into x
                 torch.index_select(x, 0, si.logit_rows[:si.num_logit_rows].long(), out=self.taps[li][:si.num_logit_rows])
@@ -639,6 +669,23 @@ class DecoderModel:
         logits = self.logits[:r]
         self._head(hl, logits)
         return logits
+
+    def _int8_layer(self, si, kv, li, lw, x, pending):
+        """A layer with 8-bit weights: both norms hand their rows on in 8 bits, and take the block's output before them onto the stream.  Returns
+        what the next norm has to add."""
+        from ..ops import int8
+
+        t, w, eps = si.num_tokens, lw.int8, self.cfg.rms_eps
+        qkv, attn, act, part = self.qkv[:t], self.attn[:t], self.act[:t], self.partial[:t]
+        rows = int8.block_norm(x, pending, pre=lw.ln1, eps=eps, int8=True)
+        if getattr(self, "tap_layers", None) and li in self.taps:
+            torch.index_select(x, 0, si.logit_rows[:si.num_logit_rows].long(), out=self.taps[li][:si.num_logit_rows])
+        int8.gemm_int8(rows, w["qkv"].q, w["qkv"].scale, bias=w["qkv_b"], out=qkv)
+        self._attention(si, kv, li, qkv, attn)
+        int8.gemm_int8(attn, w["o"].q, w["o"].scale, out=part)
+        rows = int8.block_norm(x, part, pre=lw.ln2, eps=eps, int8=True)
+        int8.gemm_int8(rows, w["gate_up"].q, w["gate_up"].scale, epilogue="swiglu", out=act)
+        return int8.gemm_int8(act, w["down"].q, w["down"].scale, out=part)
 
     def _attention(self, si, kv, li, qkv, attn):
         """Rotary embedding + KV append + paged attention of one layer over the step's rows."""
