@@ -625,6 +625,191 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 }
 
 // ----------------------------------------------------------------------------------------
+// a handful of rows in one launch
+// ----------------------------------------------------------------------------------------
+// One user's token leaves the tensor cores idle and the time is launches and latencies: two kernels, barriers, tensor memory, a cluster's sum.
+// Here every block turns the rows into 8 bits for itself, in shared memory, while its first weights are on their way, and a warp takes a
+// pair of channels (or a gate and its up channel): 16 bytes of each a lane, four products an instruction, a sum over the warp in one more.
+constexpr int kGemvThreads = 256;
+constexpr int kGemvPieces = 4;               // 16-byte pieces of each channel that a lane has in flight
+
+struct GemvParams {
+  const void* x;
+  const int8_t* q;                           // or x
+  const float* factor;
+  const int8_t* w;
+  const float* channel;
+  const float* bias;
+  const void* residual;
+  void* out;
+  long long ldx, ldq, ldw, ldr, ldc;
+  int x_elem, out_elem, x_vec, M, N, K, gated;
+};
+
+// 16 bytes of a row of weights from byte k on; what lies past its end is zero.
+OGB_DEVICE uint4 gemv_weights(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldcs(reinterpret_cast<const uint4*>(row + k));
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (k + j < K) v[j >> 2] |= (static_cast<uint32_t>(row[k + j]) & 255u) << (8 * (j & 3));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+OGB_DEVICE int dot16(const uint4& a, const uint4& b, int sum) {
+  sum = __dp4a(static_cast<int>(a.x), static_cast<int>(b.x), sum);
+  sum = __dp4a(static_cast<int>(a.y), static_cast<int>(b.y), sum);
+  sum = __dp4a(static_cast<int>(a.z), static_cast<int>(b.z), sum);
+  return __dp4a(static_cast<int>(a.w), static_cast<int>(b.w), sum);
+}
+
+// ROWS: rows held, at least M.
+template <int ROWS>
+__global__ void __launch_bounds__(kGemvThreads, 3) gemv_int8_kernel(const GemvParams p) {
+  extern __shared__ __align__(16) int8_t codes[];                  // [ROWS][K to a multiple of 16]
+  __shared__ uint32_t part[kGemvThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = gridDim.x * (kGemvThreads / 32);
+  const int pitch = (p.K + 15) / 16 * 16, n_out = p.gated != 0 ? p.N / 2 : p.N;
+  const int pairs = p.gated != 0 ? n_out : (p.N + 1) / 2;
+  int pair = blockIdx.x * (kGemvThreads / 32) + warp;
+  auto rows_of = [&](int i, int& a, int& b) {
+    if (p.gated != 0) {
+      a = (i >> 7) * 256 + (i & 127);
+      b = a + 128;
+    } else {
+      a = 2 * i;
+      b = min(a + 1, p.N - 1);
+    }
+  };
+  uint4 wa[kGemvPieces], wb[kGemvPieces];
+  auto fetch = [&](int i, int k0) {
+    int a, b;
+    rows_of(i, a, b);
+#pragma unroll
+    for (int u = 0; u < kGemvPieces; ++u) {
+      const int k = k0 + (u * 32 + lane) * 16;
+      if (k < p.K) {
+        wa[u] = gemv_weights(p.w + static_cast<size_t>(a) * p.ldw, k, p.K);
+        wb[u] = gemv_weights(p.w + static_cast<size_t>(b) * p.ldw, k, p.K);
+      }
+    }
+  };
+  pdl_trigger();
+  if (pair < pairs) fetch(pair, 0);
+  pdl_wait();
+
+  // ---- rows to codes ----
+  const void* x = after_wait(p.x);
+  const int8_t* q = after_wait(p.q);
+  float s[ROWS];
+  if (q == nullptr) {
+    // all rows at once, an equal share of the warps each
+    constexpr int kWarps = kGemvThreads / 32 / ROWS, kLanes = 32 * kWarps;
+    const int m = warp / kWarps, t = tid - m * kLanes;
+    const size_t row = static_cast<size_t>(m) * p.ldx;
+    uint32_t peak = 0;
+    if (m < p.M) {
+#pragma unroll 4
+      for (int i = t * 8; i < p.K; i += kLanes * 8) {
+        float f[8];
+        load8(x, p.x_elem, p.x_vec != 0, row, i, p.K, f);
+        peak = max(peak, peak_bits8(f));
+      }
+    }
+    peak = __reduce_max_sync(0xffffffffu, peak);
+    if (lane == 0) part[warp] = peak;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = max(top, part[r * kWarps + w]);
+      const RowCode code(top);
+      s[r] = code.factor;
+      if (r == m && m < p.M) {
+#pragma unroll 2
+        for (int i = t * 8; i < p.K; i += kLanes * 8) {
+          float f[8];
+          load8(x, p.x_elem, p.x_vec != 0, row, i, p.K, f);
+          store_codes(codes, static_cast<size_t>(m) * pitch, i, p.x_elem == kElemF32 ? code.codes(f) : code.codes_short(f));
+        }
+      }
+    }
+  } else {
+    const float* factor = after_wait(p.factor);
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+      if (m < p.M) {
+        s[m] = factor[m];
+        for (int i = tid * 16; i < p.K; i += kGemvThreads * 16)
+          *reinterpret_cast<uint4*>(codes + static_cast<size_t>(m) * pitch + i) = gemv_weights(q + static_cast<size_t>(m) * p.ldq, i, p.K);
+      }
+  }
+  // store_codes writes eight at a time: the last eight of the pitch may be nobody's
+  if (q == nullptr && tid < ROWS && pitch - (p.K + 7) / 8 * 8 == 8 && tid < p.M)
+    *reinterpret_cast<uint2*>(codes + static_cast<size_t>(tid) * pitch + pitch - 8) = make_uint2(0, 0);
+  __syncthreads();
+
+  for (; pair < pairs; pair += warps) {
+    int sum_a[ROWS], sum_b[ROWS];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) sum_a[m] = sum_b[m] = 0;
+    for (int k0 = 0; k0 < p.K; k0 += kGemvPieces * 512) {
+#pragma unroll
+      for (int u = 0; u < kGemvPieces; ++u) {
+        const int k = k0 + (u * 32 + lane) * 16;
+        if (k < p.K) {
+#pragma unroll
+          for (int m = 0; m < ROWS; ++m)
+            if (m < p.M) {
+              const uint4 c = *reinterpret_cast<const uint4*>(codes + static_cast<size_t>(m) * pitch + k);
+              sum_a[m] = dot16(wa[u], c, sum_a[m]);
+              sum_b[m] = dot16(wb[u], c, sum_b[m]);
+            }
+        }
+      }
+      // the next pieces: of this pair, or of the next one
+      if (k0 + kGemvPieces * 512 < p.K) fetch(pair, k0 + kGemvPieces * 512);
+      else if (pair + warps < pairs) fetch(pair + warps, 0);
+    }
+    int a, b;
+    rows_of(pair, a, b);
+    const float ca = __ldg(p.channel + a), cb = __ldg(p.channel + b);
+    const float ba = p.bias != nullptr ? __ldg(p.bias + a) : 0.f, bb = p.bias != nullptr ? __ldg(p.bias + b) : 0.f;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      sum_a[m] = __reduce_add_sync(0xffffffffu, sum_a[m]);
+      sum_b[m] = __reduce_add_sync(0xffffffffu, sum_b[m]);
+      if (m >= p.M || lane != m) continue;                        // a lane a row
+      float va = fmaf(static_cast<float>(sum_a[m]) * s[m], ca, ba), vb = fmaf(static_cast<float>(sum_b[m]) * s[m], cb, bb);
+      const size_t at = static_cast<size_t>(m) * p.ldc, from = static_cast<size_t>(m) * p.ldr;
+      if (p.gated != 0) {
+        store_elem(p.out, p.out_elem, at + pair, __fdividef(va, 1.f + __expf(-va)) * vb);
+        continue;
+      }
+      if (p.residual != nullptr) {
+        va += load_elem(p.residual, p.out_elem, from + a);
+        vb += load_elem(p.residual, p.out_elem, from + b);
+      }
+      store_elem(p.out, p.out_elem, at + a, va);
+      if (2 * pair + 1 < p.N) store_elem(p.out, p.out_elem, at + b, vb);
+    }
+  }
+}
+
+// Rows and sizes that this kernel takes (times in us with weights from HBM, tensor cores -> this one).  One row: 1152 x 896 7.8 -> 3.2, 4608 x 3584 11.5 ->
+// 7.4, gated 9728 x 896 8.8 -> 5.9, 20000 x 2048 16.2 -> 12.8; but 37888 x 3584 26.7 -> 34.7 and 3584 x 11008, whose blocks all round a long
+// row, 15.6 -> 19.3.  Two: 3584 x 3584 10.4 -> 9.3, 20000 x 2048 16.2 -> 14.7.  Four: 4608 x 3584 11.6 -> 14.1.
+static bool gemv_applies(int M, int N, int K) { return M <= 2 && M * K <= 8192 && static_cast<long long>(N) * K <= (48ll << 20); }
+
+template <int ROWS>
+static int launch_gemv(const GemvParams& p, cudaStream_t stream) {
+  const int smem = ROWS * ((p.K + 15) / 16 * 16);
+  const int pairs = p.gated != 0 ? p.N / 2 : (p.N + 1) / 2;
+  const int grid = std::min((pairs + kGemvThreads / 32 - 1) / (kGemvThreads / 32), 3 * ogb_num_sms());
+  return static_cast<int>(launch_overlapped(gemv_int8_kernel<ROWS>, dim3(grid), dim3(kGemvThreads), smem, stream, p));
+}
+
+// ----------------------------------------------------------------------------------------
 // host side
 // ----------------------------------------------------------------------------------------
 // How a product is divided, from its sizes alone.
@@ -730,6 +915,7 @@ static long long i8_factor_bytes(int M) { return (static_cast<long long>(M) * 4 
 
 extern "C" int64_t ogb_gemm_int8_workspace(int M, int N, int K, int gated, int quantize) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (gemv_applies(M, N, K)) return 0;
   const Int8Plan plan = i8_plan(M, N, K, gated != 0, ogb_num_sms());
   return plan.counter_bytes + plan.ws_bytes + (quantize != 0 ? i8_rows_bytes(M, K) + i8_factor_bytes(M) : 0);
 }
@@ -744,9 +930,14 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
   if (q != nullptr && ((ldq & 15) != 0 || ldq < K || (reinterpret_cast<uintptr_t>(q) & 15) != 0)) return -4;
   if (gated != 0 && (N % 256) != 0) return -6;
   if (static_cast<long long>((M + 15) / 16) * ((N + 127) / 128) > (1 << 30)) return -2;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (gemv_applies(M, N, K)) {
+    const GemvParams p{x, static_cast<const int8_t*>(q), factor, static_cast<const int8_t*>(w), channel, bias, residual, out, ldx, ldq, ldw, ldr, ldc,
+                       x_elem, out_elem, rows_aligned(x, ldx, x_elem), M, N, K, gated};
+    return M == 1 ? launch_gemv<1>(p, stream) : launch_gemv<2>(p, stream);
+  }
   const int sms = ogb_num_sms();
   const Int8Plan plan = i8_plan(M, N, K, gated != 0, sms);
-  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool quantize = q == nullptr;
   const long long rows_bytes = quantize ? i8_rows_bytes(M, K) : 0, factor_bytes = quantize ? i8_factor_bytes(M) : 0;
   if (ws_bytes < rows_bytes + factor_bytes + plan.counter_bytes + plan.ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 255) != 0) return -8;
@@ -783,4 +974,13 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
   if (out_elem == kElemF32) return launch_int8<1, kElemF32>(plan, p, q, ldq, w, ldw, K, early, stream);
   if (out_elem == kElemBf16) return launch_int8<1, kElemBf16>(plan, p, q, ldq, w, ldw, K, early, stream);
   return launch_int8<1, kElemF16>(plan, p, q, ldq, w, ldw, K, early, stream);
+}
+
+// The same call with its arguments as 64-bit words in their order: a binding that converts every argument by itself spends as long on these as on a
+// launch.
+extern "C" int ogb_gemm_int8_args(const int64_t* a) {
+  auto p = [&](int i) { return reinterpret_cast<void*>(a[i]); };
+  auto n = [&](int i) { return static_cast<int>(a[i]); };
+  return ogb_gemm_int8(p(0), n(1), a[2], p(3), static_cast<const float*>(p(4)), a[5], p(6), a[7], static_cast<const float*>(p(8)), static_cast<const float*>(p(9)),
+                       p(10), a[11], p(12), a[13], n(14), n(15), n(16), n(17), n(18), p(19), a[20], static_cast<int*>(p(21)), p(22));
 }

@@ -10,6 +10,7 @@
 // block of as many threads as leave each at most kNormVec pieces of eight values.  Few rows (a decode step) take a piece a thread, as
 // the time is then a chain of latencies -- load, three sums over the row, store -- and not bandwidth.
 #include <stdint.h>
+#include <string.h>
 
 #include <algorithm>
 
@@ -557,4 +558,13 @@ extern "C" int ogb_block_norm(const void* x, const void* y, const void* gate, co
   if (t == 32) return launch_norm<2, 32>(p, t, stream);
   if (pieces <= t) return launch_norm<1, kMostThreads>(p, t, stream);
   return pieces <= 2 * t ? launch_norm<2, kMostThreads>(p, t, stream) : launch_norm<kVec, kMostThreads>(p, t, stream);
+}
+
+// The same call with its arguments as 64-bit words, floating ones as doubles: see ogb_gemm_int8_args.
+extern "C" int ogb_block_norm_args(const int64_t* a) {
+  auto p = [&](int i) { return reinterpret_cast<void*>(a[i]); };
+  auto n = [&](int i) { return static_cast<int>(a[i]); };
+  auto f = [&](int i) { double d; memcpy(&d, a + i, 8); return static_cast<float>(d); };
+  return ogb_block_norm(p(0), p(1), p(2), p(3), p(4), p(5), p(6), p(7), static_cast<float*>(p(8)), a[9], a[10], a[11], a[12], a[13], a[14], n(15), n(16), n(17),
+                        n(18), n(19), n(20), n(21), n(22), f(23), f(24), f(25), p(26));
 }

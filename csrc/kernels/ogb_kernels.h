@@ -279,6 +279,9 @@ int ogb_block_norm(const void* x, const void* y, const void* gate, const void* p
                    float* factor, int64_t ldx, int64_t ldy, int64_t ldg, int64_t ldxo, int64_t ldh, int64_t ldq, int rows, int cols,
                    int x_elem, int y_elem, int gate_elem, int w_elem, int h_elem, int gate_sigmoid, float eps, float x_scale, float y_scale,
                    void* stream);
+// The two with their arguments as 64-bit words in their order, floating ones as doubles.
+int ogb_gemm_int8_args(const int64_t* args);
+int ogb_block_norm_args(const int64_t* args);
 // Per row of logits: log probability of tokens[row] (a negative token asks for none: 0, rank -1), entropy (or null), rank (or null), the `top` likeliest (up
 // to 32) with theirs.
 int ogb_token_logprobs(const void* logits, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,

@@ -43,14 +43,19 @@ def _stream() -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def current_index() -> int:
-    """Index of the current CUDA device (CUDA has to be up)."""
-    return torch.cuda.current_device()
+# Index of the current device, where CUDA is up (a CUDA tensor is at hand).
+current_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def status_ptr(index: int) -> int:
+    """Address of the status word of CUDA device ``index``."""
+    w = _status_words.get(index)
+    return (status_word(index) if w is None else w).data_ptr()
 
 
 def status_word(device=None) -> torch.Tensor:
     """Per-device int32 word kernels OR error bits into (wait timeout, index out of range...)."""
-    idx = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    idx = torch.cuda.current_device() if device is None else torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index or 0
     w = _status_words.get(idx)
     if w is None:
         w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
@@ -554,6 +559,7 @@ class TokenLogprobs(NamedTuple):
 
 
 _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TOKEN_TYPES = (torch.int32, torch.int64)
 MAX_TOP_LOGPROBS = 32
 MAX_VOCAB, MAX_VOCAB_WITH_TOP = 1 << 30, 3_000_000
 
@@ -566,36 +572,42 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
     A negative token asks for none: log probability 0 and rank -1.  A token past the vocabulary raises the status word's index bit, with NaN and
     rank -1.  Logits of minus infinity weigh nothing; a row of nothing else, or with a NaN or plus infinity, has NaN for log probabilities and entropy (among the
     likeliest, NaN comes last)."""
-    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES or logits.shape[1] < 1:
-        raise ValueError(f"logits: a matrix of fp32, bf16 or fp16, not {tuple(logits.shape)} {logits.dtype}")
-    rows, vocab = logits.shape
-    if not 0 <= top <= min(MAX_TOP_LOGPROBS, vocab):
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    shape = logits.shape
+    if kind is None or len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"logits: a matrix of fp32, bf16 or fp16, not {tuple(shape)} {logits.dtype}")
+    rows, vocab = shape
+    if not 0 <= top <= (MAX_TOP_LOGPROBS if vocab > MAX_TOP_LOGPROBS else vocab):
         raise ValueError(f"top = {top}: between 0 and {min(MAX_TOP_LOGPROBS, vocab)}")
-    if vocab > MAX_VOCAB or (top and vocab > MAX_VOCAB_WITH_TOP):
+    if vocab > MAX_VOCAB_WITH_TOP and (top or vocab > MAX_VOCAB):
         raise ValueError(f"a vocabulary of {vocab}: at most {MAX_VOCAB_WITH_TOP if top else MAX_VOCAB}")
-    if tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
+    dev = logits.device
+    if tokens.shape != (rows,) or tokens.device != dev or tokens.dtype not in _TOKEN_TYPES:
         raise ValueError(f"tokens: {rows} whole numbers (int32, int64) on the device of the logits")
     if not logits.is_cuda:
         return TokenLogprobs(*reference.token_logprobs(logits, tokens, top, entropy))
-    if vocab > 1 and logits.stride(1) != 1:
-        logits = logits.contiguous()
-    if tokens.dtype != torch.int32:
+    ld, step = logits.stride()
+    if step != 1 and vocab > 1:
+        logits, ld = logits.contiguous(), vocab
+    if tokens.dtype is not torch.int32:
         tokens = tokens.clamp(-1, 2**31 - 1).int()         # what is past 32 bits stays past the vocabulary
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    dev = logits.device
     index = dev.index
     if index != current_index():
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, entropy)
     logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    rank = torch.empty(rows, dtype=torch.int32, device=dev)
-    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
-    ids = torch.empty(rows, top, dtype=torch.int32, device=dev) if top else None
-    lps = torch.empty(rows, top, dtype=torch.float32, device=dev) if top else None
+    rank = torch.empty_like(tokens)
+    ent = torch.empty_like(logprob) if entropy else None
+    ids = lps = None
+    if top:
+        # (a matrix by its strides: torch.empty takes twice as long for two dimensions as for one)
+        ids = torch.empty_strided((rows, top), (top, 1), dtype=torch.int32, device=dev)
+        lps = torch.empty_like(ids, dtype=torch.float32)
     rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ent.data_ptr() if entropy else 0, rank.data_ptr(),
-                                           ids.data_ptr() if top else 0, lps.data_ptr() if top else 0, rows, vocab, logits.stride(0), top,
-                                           _LOGIT_TYPES[logits.dtype], status_word(dev).data_ptr(), _raw_stream(index))
+                                           ids.data_ptr() if top else 0, lps.data_ptr() if top else 0, rows, vocab, ld, top, kind, status_ptr(index),
+                                           _raw_stream(index))
     _native.check(rc, "ogb_token_logprobs")
     launch_counts["token_logprobs"] += 1
     return TokenLogprobs(logprob, rank, ent, ids, lps)

@@ -8,14 +8,18 @@ the statements of :mod:`onnx_genai_b200.ops.reference`.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
+import struct
 from typing import NamedTuple
 
 import torch
 
-from . import _native, _raw_stream, _timed, current_index, launch_counts, reference, status_word
+from . import _native, _raw_stream, _timed, current_index, launch_counts, reference, status_ptr
 
 P, I, L, F = _native.P, _native.I, _native.L, _native.F
+_native.register("ogb_gemm_int8_args", [ctypes.c_char_p])
+_native.register("ogb_block_norm_args", [ctypes.c_char_p])
 _native.register("ogb_quantize_rows", [P] * 3 + [I] * 2 + [L] * 2 + [I, P])
 _native.register("ogb_gemm_int8_workspace", [I] * 5, L)
 _native.register("ogb_gemm_int8", [P, I, L, P, P, L, P, L, P, P, P, L, P, L] + [I] * 5 + [P, L, P, P])
@@ -25,6 +29,9 @@ ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_K = 131072          # sums of 128 * 127 * K stay below 2^31
 MAX_HIDDEN = 16384      # a row of block_norm stays in registers
 _EPI = ("none", "residual", "swiglu")
+# arguments of the two calls with many, as 64-bit words (ctypes takes 2 us to convert them one by one)
+_pack_gemm = struct.Struct("23q").pack
+_pack_norm = struct.Struct("23q3dq").pack
 
 
 class Int8Rows(NamedTuple):
@@ -42,9 +49,11 @@ def _refuse(what):
 
 def _padded(rows, k, device):
     """[rows, k] int8 whose rows begin at multiples of 16 bytes."""
-    if k % 16 == 0:
-        return torch.empty(rows, k, dtype=torch.int8, device=device)
-    return torch.empty(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :k]
+    pitch = (k + 15) // 16 * 16
+    if pitch == k:
+        # (by its strides: torch.empty takes twice as long for two dimensions as for one)
+        return torch.empty_strided((rows, k), (k, 1), dtype=torch.int8, device=device)
+    return torch.empty(rows, pitch, dtype=torch.int8, device=device)[:, :k]
 
 
 @_timed("quantize_rows")
@@ -108,30 +117,37 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     gated = epilogue == "swiglu"
     if epilogue not in _EPI:
         _refuse(f"epilogue {epilogue!r}: one of {', '.join(_EPI)}")
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
-        _refuse(f"a {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
-    m, k = x.shape
-    n, dev = w.shape[0], x.device
-    if (x.dtype != torch.int8) if rows else (x.dtype not in ELEM):
-        _refuse(f"rows of {x.dtype}")
+    shape, wshape = x.shape, w.shape
+    if len(shape) != 2 or len(wshape) != 2 or shape[1] != wshape[1]:
+        _refuse(f"a {tuple(shape)} and w {tuple(wshape)} do not multiply")
+    m, k = shape
+    n, dev, dtype = wshape[0], x.device, x.dtype
+    kind = ELEM.get(dtype, 0) if rows else ELEM.get(dtype)
+    if (dtype is not torch.int8) if rows else (kind is None):
+        _refuse(f"rows of {dtype}")
     if not 0 < k <= MAX_K:
         _refuse(f"k = {k}: between 1 and {MAX_K}")
-    if w.dtype != torch.int8 or w.device != dev:
+    if w.dtype is not torch.int8 or w.device != dev:
         _refuse("w must be int8 on the device of a")
     if w_scale is None or not _channels(w_scale, n, dev) or not (bias is None or _channels(bias, n, dev)):
         _refuse(f"w_scale and bias: {n} contiguous fp32 values each on the device of a")
-    if gated and (n % 256 or residual is not None):
-        _refuse("swiglu takes a weight of quantize_gate_up and no residual")
-    if epilogue == "residual" and residual is None:
-        _refuse("the residual is missing")
-    n_out = n // 2 if gated else n
+    n_out = n
+    if gated:
+        if n % 256 or residual is not None:
+            _refuse("swiglu takes a weight of quantize_gate_up and no residual")
+        n_out = n // 2
+    elif residual is None:
+        if epilogue == "residual":
+            _refuse("the residual is missing")
     if out_dtype is None:
-        out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16 if rows else x.dtype
-    if out_dtype not in ELEM:
+        out_dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.bfloat16 if rows else dtype
+    out_kind = ELEM.get(out_dtype)
+    if out_kind is None:
         _refuse(f"results of {out_dtype}")
-    for t in (out, residual):
-        if t is not None and (t.shape != (m, n_out) or t.dtype != out_dtype or t.device != dev or (n_out > 1 and t.stride(1) != 1)):
-            _refuse(f"out and residual: [{m}, {n_out}] {out_dtype} with neighbouring columns on the device of a")
+    if out is not None:
+        _result(out, m, n_out, out_dtype, dev)
+    if residual is not None:
+        _result(residual, m, n_out, out_dtype, dev)
     if not x.is_cuda:
         y = reference.gemm_int8(a, w, w_scale, bias, residual, gated, out_dtype)
         return y if out is None else out.copy_(y)
@@ -141,41 +157,50 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
         ldw = (k + 15) // 16 * 16
     if m == 1:
         ldx = (k + 15) // 16 * 16
-    if out is not None and m > 1 and out.stride(0) < n_out:
-        _refuse("rows of out overlap")
-    if (c1 != 1 and k > 1) or ldw % 16 or w.data_ptr() % 16 or ldw < k:
+    x_ptr, w_ptr = x.data_ptr(), w.data_ptr()
+    if (c1 != 1 and k > 1) or ldw % 16 or w_ptr % 16 or ldw < k:
         _refuse("rows of w must begin at multiples of 16 bytes: lay it out by quantize_weight")
     if rows:
-        if (x1 != 1 and k > 1) or ldx % 16 or x.data_ptr() % 16 or ldx < k:
+        if (x1 != 1 and k > 1) or ldx % 16 or x_ptr % 16 or ldx < k:
             _refuse("8-bit rows must begin at multiples of 16 bytes")
         if not _channels(a.scale, m, dev):
             _refuse("a.scale: a contiguous fp32 value a row on the device of a.q")
     elif x1 != 1 and k > 1:
         x = x.contiguous()
-        ldx = k
+        x_ptr, ldx = x.data_ptr(), k
     index = dev.index
     if index != current_index():
         with torch.cuda.device(index):
             return gemm_int8(a, w, w_scale, bias, residual, epilogue, out, out_dtype)
     if out is None:
-        out = torch.empty(m, n_out, dtype=out_dtype, device=dev)
+        out = torch.empty_strided((m, n_out), (n_out, 1), dtype=out_dtype, device=dev)
+        ldc = n_out
+    else:
+        ldc = out.stride(0)
+        if m > 1 and ldc < n_out:
+            _refuse("rows of out overlap")
     if m == 0 or n == 0:
         return out
     # the caller's own memory for as long as the call: the allocator hands it on in the stream's order, and a captured graph keeps its own
     size = _workspace(m, n, k, gated, not rows)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    rc = _native.load().ogb_gemm_int8(0 if rows else x.data_ptr(), 0 if rows else ELEM[x.dtype], ldx, x.data_ptr() if rows else 0,
-                                      a.scale.data_ptr() if rows else 0, ldx, w.data_ptr(), ldw, w_scale.data_ptr(),
-                                      0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                                      0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0), ELEM[out_dtype], m, n, k, gated,
-                                      ws.data_ptr() if size else 0, size, status_word(dev).data_ptr(), _raw_stream(index))
-    _native.check(rc, "ogb_gemm_int8")
+    rc = _native.load().ogb_gemm_int8_args(_pack_gemm(
+        0 if rows else x_ptr, kind, ldx, x_ptr if rows else 0, a.scale.data_ptr() if rows else 0, ldx, w_ptr, ldw, w_scale.data_ptr(),
+        0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0),
+        out.data_ptr(), ldc, out_kind, m, n, k, gated, 0 if ws is None else ws.data_ptr(), size, status_ptr(index), _raw_stream(index)))
+    if rc:
+        _native.check(rc, "ogb_gemm_int8")
     launch_counts["gemm_int8"] += 1
     return out
 
 
+def _result(t, m, n, dtype, dev):
+    if t.shape != (m, n) or t.dtype is not dtype or t.device != dev or (n > 1 and t.stride(1) != 1):
+        _refuse(f"out and residual: [{m}, {n}] {dtype} with neighbouring columns on the device of a")
+
+
 def _channels(t, n, dev):
-    return t.dtype == torch.float32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == dev
+    return t.dtype is torch.float32 and t.shape == (n,) and t.device == dev and t.is_contiguous()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -194,39 +219,57 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     type (None: no norm).  ``gate``: [hidden] or [rows, hidden], taken as it is or through a sigmoid.  ``h`` comes in ``out_dtype`` (that of ``out``, else of ``x``), or as
     :class:`Int8Rows` with ``int8=True``.  All of it is computed in 32 bits and rounded where it is stored; h is taken from x' before that is
     rounded.  ``hidden`` is at most 16384 on CUDA; the tensors' columns are neighbours."""
-    if x.dim() != 2 or x.dtype not in ELEM:
-        _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(x.shape)} {x.dtype}")
-    shape, dev = x.shape, x.device
+    shape, dev, dtype = x.shape, x.device, x.dtype
+    kind = ELEM.get(dtype)
+    if kind is None or len(shape) != 2:
+        _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(shape)} {dtype}")
     rows, n = shape
     if n == 0:
         _refuse("rows without values")
-    if x.stride(1) != 1 and n > 1:
-        _refuse("x: neighbouring columns")
-    wide = gate is not None and gate.dim() == 2
-    for t in (y, x_out, out, gate if wide else None):
-        if t is not None and (t.shape != shape or t.dtype not in ELEM or t.device != dev or (t.stride(1) != 1 and n > 1)):
-            _refuse("y, x_out, out and a gate for each token: matrices of x's shape and device with neighbouring columns")
-    for t in (post, pre, None if wide else gate):
-        if t is not None and (t.dim() != 1 or t.shape[0] != n or t.dtype not in ELEM or t.device != dev or not t.is_contiguous()):
-            _refuse(f"post, pre and a gate for each channel: {n} contiguous values on x's device")
-    if y is None and (post is not None or gate is not None):
+    ldx = _matrix(x, shape, dev)
+    ldy = ldg = ldo = 0
+    y_kind = gate_kind = w_kind = 0
+    y_ptr = gate_ptr = post_ptr = pre_ptr = new_ptr = 0
+    if y is not None:
+        ldy, y_kind, y_ptr = _matrix(y, shape, dev), ELEM[y.dtype], y.data_ptr()
+    elif post is not None or gate is not None:
         _refuse("a post norm or a gate needs y")
-    if post is not None and pre is not None and post.dtype != pre.dtype:
-        _refuse("post and pre weights have one type")
-    if x_out is not None and x_out.dtype != x.dtype:
-        _refuse("x_out has the type of x")
-    for t in (x_out if x_out is not None else x, out):
-        if t is not None and rows > 1 and t.stride(0) < n:
-            _refuse("rows of x_out (or x, where it takes the new stream) and out do not overlap")
+    if gate is not None:
+        if gate.dim() == 2:
+            ldg = _matrix(gate, shape, dev)
+        else:
+            _vector(gate, n, dev)
+        gate_kind, gate_ptr = ELEM[gate.dtype], gate.data_ptr()
+    if post is not None:
+        _vector(post, n, dev)
+        w_kind, post_ptr = ELEM[post.dtype], post.data_ptr()
+    if pre is not None:
+        _vector(pre, n, dev)
+        if post is not None and post.dtype is not pre.dtype:
+            _refuse("post and pre weights have one type")
+        w_kind, pre_ptr = ELEM[pre.dtype], pre.data_ptr()
+    ldn = ldx
+    if x_out is not None:
+        if x_out.dtype is not dtype:
+            _refuse("x_out has the type of x")
+        ldn = _matrix(x_out, shape, dev)
+    elif y is not None or x_scale != 1.0:
+        x_out = x
+    if x_out is not None:
+        if ldn < n and rows > 1:
+            _refuse("rows of x_out (or x, where it takes the new stream) overlap")
+        new_ptr = x_out.data_ptr()
     if int8:
         if out is not None or out_dtype is not None:
             _refuse("8-bit rows are made by the call")
     else:
-        out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-        if out_dtype not in ELEM or (out is not None and out.dtype != out_dtype):
+        out_dtype = out_dtype or (out.dtype if out is not None else dtype)
+        if out_dtype not in ELEM or (out is not None and out.dtype is not out_dtype):
             _refuse(f"results of {out_dtype}")
-    if x_out is None and (y is not None or x_scale != 1.0):
-        x_out = x
+        if out is not None:
+            ldo = _matrix(out, shape, dev)
+            if ldo < n and rows > 1:
+                _refuse("rows of out overlap")
     if not x.is_cuda:
         new, h = reference.block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid)
         if int8:
@@ -245,19 +288,31 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     if index != current_index():
         with torch.cuda.device(index):
             return block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid, x_out, out, None if int8 else out_dtype, int8)
-    q = scale = None
     if int8:
         q, scale = _padded(rows, n, dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    elif out is None:
-        out = torch.empty(rows, n, dtype=out_dtype, device=dev)
-    weight = post if post is not None else pre
-    rc = _native.load().ogb_block_norm(
-        x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if gate is None else gate.data_ptr(), 0 if post is None else post.data_ptr(),
-        0 if pre is None else pre.data_ptr(), 0 if x_out is None else x_out.data_ptr(), 0 if out is None else out.data_ptr(),
-        q.data_ptr() if int8 else 0, scale.data_ptr() if int8 else 0, x.stride(0), 0 if y is None else y.stride(0), gate.stride(0) if wide else 0,
-        0 if x_out is None else x_out.stride(0), 0 if out is None else out.stride(0), q.stride(0) if int8 else 0, rows, n, ELEM[x.dtype],
-        0 if y is None else ELEM[y.dtype], 0 if gate is None else ELEM[gate.dtype], 0 if weight is None else ELEM[weight.dtype],
-        0 if out is None else ELEM[out_dtype], gate_sigmoid, eps, x_scale, y_scale, _raw_stream(index))
-    _native.check(rc, "ogb_block_norm")
+        q_ptr, ldq, scale_ptr, out_ptr, out_kind = q.data_ptr(), (n + 15) // 16 * 16, scale.data_ptr(), 0, 0
+    else:
+        if out is None:
+            out, ldo = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=dev), n
+        q_ptr = ldq = scale_ptr = 0
+        out_ptr, out_kind = out.data_ptr(), ELEM[out_dtype]
+    rc = _native.load().ogb_block_norm_args(_pack_norm(x.data_ptr(), y_ptr, gate_ptr, post_ptr, pre_ptr, new_ptr, out_ptr, q_ptr, scale_ptr, ldx, ldy, ldg, ldn, ldo,
+                                                       ldq, rows, n, kind, y_kind, gate_kind, w_kind, out_kind, gate_sigmoid, eps, x_scale, y_scale,
+                                                       _raw_stream(index)))
+    if rc:
+        _native.check(rc, "ogb_block_norm")
     launch_counts["block_norm"] += 1
     return Int8Rows(q, scale) if int8 else out
+
+
+def _matrix(t, shape, dev):
+    """Stride of the rows of a matrix that goes with x."""
+    ld, step = t.stride() if t.dim() == 2 else (0, 0)
+    if t.shape != shape or t.dtype not in ELEM or t.device != dev or (step != 1 and shape[1] > 1):
+        _refuse("x, y, x_out, out and a gate for each token: matrices of one shape, fp32, bf16 or fp16, on one device, with neighbouring columns")
+    return ld
+
+
+def _vector(t, n, dev):
+    if t.shape != (n,) or t.dtype not in ELEM or t.device != dev or not t.is_contiguous():
+        _refuse(f"post, pre and a gate for each channel: {n} contiguous values on x's device")
