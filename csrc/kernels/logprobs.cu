@@ -181,6 +181,7 @@ struct LpShared {
   LpState part[kLpWarps];
   int rank_part[kLpWarps];
   int count, reach;
+  int pieces[kLpQuick];
   LpState total;
   int rank_total;
 };
@@ -223,9 +224,9 @@ OGB_DEVICE void lp_load(const T* x, int i0, int vocab, uint32_t (&w)[8]) {
 }
 
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobsParams p) {
+__global__ void __launch_bounds__(kLpThreads, TOP ? 4 : 5) logprobs_kernel(const LogprobsParams p) {
   using Type = LpType<T>;
-  constexpr int kPer = Type::kPer, kUnroll = TOP ? 2 : 4;       // 32-byte pieces that a thread has in flight, as registers allow
+  constexpr int kPer = Type::kPer, kUnroll = 1;                   // 32-byte pieces a round
   __shared__ LpShared<T> sh;
   extern __shared__ __align__(16) uint8_t dynamic_smem[];
   typename Type::Max* piece_max = reinterpret_cast<typename Type::Max*>(dynamic_smem);
@@ -249,11 +250,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobsP
   Float2 s2(0.f), t2(0.f);
   int rank = 0;
   const Float2 log2e(1.4426950408889634f);
+  // the next pieces are on their way while these are summed
+  uint32_t next[kUnroll][8];
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u * kLpThreads < n_pieces) lp_load(x, first + (b + u * kLpThreads) * kPer, p.vocab, next[u]);
+  };
+  fetch(tid);
   for (int b = tid; b < n_pieces; b += kLpThreads * kUnroll) {
     uint32_t w[kUnroll][8];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (b + u * kLpThreads < n_pieces) lp_load(x, first + (b + u * kLpThreads) * kPer, p.vocab, w[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[u][j] = next[u][j];
+    fetch(b + kLpThreads * kUnroll);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int piece = b + u * kLpThreads;
@@ -353,16 +364,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobsP
     unsigned long long floor_key = sh.bound != 0 ? sh.bound - 1 : 0;          // fewer threads than `top` have a value: every value may be one
     const float floor_value = lp_value(floor_key + 1);
     auto reaches = [&](int b) { return !(lp_float(piece_max[b]) < floor_value) && upper(b) > floor_key; };
-    int mine = 0;
-    for (int b = tid; b < n_pieces; b += kLpThreads) mine += reaches(b) ? 1 : 0;
-    if (mine != 0) atomicAdd(&sh.reach, mine);
+    for (int b = tid; b < n_pieces; b += kLpThreads)
+      if (reaches(b)) {
+        const int at = atomicAdd(&sh.reach, 1);
+        if (at < kLpQuick) sh.pieces[at] = b;
+      }
     __syncthreads();
     if (sh.reach <= kLpQuick) {
-      for (int b = tid; mine != 0; b += kLpThreads)
-        if (reaches(b)) {
-          add_piece(b, floor_key);
-          --mine;
+      // a value a thread, all of them at one latency
+      for (int e = tid; e < sh.reach * kPer; e += kLpThreads) {
+        const int i = first + sh.pieces[e / kPer] * kPer + e % kPer;
+        if (i >= 0 && i < p.vocab) {
+          const unsigned long long key = lp_key(load_elem(x, Type::kElem, i), i);
+          if (key > floor_key) sh.keys[atomicAdd(&sh.count, 1)] = key;
         }
+      }
       __syncthreads();
       if (sh.count <= kLpMaxTop) held = sh.count;           // the join puts them in order
       else keep_best(floor_key);

@@ -598,13 +598,13 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
         with torch.cuda.device(index):
             return token_logprobs(logits, tokens, top, entropy)
     logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    rank = torch.empty_like(tokens)
-    ent = torch.empty_like(logprob) if entropy else None
+    rank = torch.empty(rows, dtype=torch.int32, device=dev)
+    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
     ids = lps = None
     if top:
         # (a matrix by its strides: torch.empty takes twice as long for two dimensions as for one)
         ids = torch.empty_strided((rows, top), (top, 1), dtype=torch.int32, device=dev)
-        lps = torch.empty_like(ids, dtype=torch.float32)
+        lps = torch.empty_strided((rows, top), (top, 1), dtype=torch.float32, device=dev)
     rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ent.data_ptr() if entropy else 0, rank.data_ptr(),
                                            ids.data_ptr() if top else 0, lps.data_ptr() if top else 0, rows, vocab, ld, top, kind, status_ptr(index),
                                            _raw_stream(index))
