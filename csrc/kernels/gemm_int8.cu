@@ -52,7 +52,7 @@ struct Int8Params {
   int n_tiles, m_tiles, tiles, k_blocks, stages;
   int splits;                                // CTAs (a cluster) per tile; 0: whole tiles and ranges
   int cut;                                   // the first `cut` tiles are cut into ranges of
-  int range, longer;                         //   `range` k-blocks a CTA, and one more for the first `longer`
+  int range, longer;                         //   `range` k-blocks a CTA, and one more for the first `longer`; of a cluster's tile likewise
   int* status;
   int* ws;                                   // [CTA][2][TW][4 quarters][rows / 4][32 channels][4 rows]
   unsigned int* counters;                    // [CTA], zero when the kernel starts
@@ -76,12 +76,22 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 // Tiles in groups of kI8Group tiles of W: within a group W goes fastest, so that the tiles under way at one time (about 148) share both operands
 // in L2.
 OGB_DEVICE void i8_tile(const Int8Params& p, int tile, int& nt, int& mt) {
+  if (p.m_tiles == 1) {
+    nt = tile;
+    mt = 0;
+    return;
+  }
   const int g = tile / (kI8Group * p.m_tiles), first = g * kI8Group;
   const int wide = min(kI8Group, p.n_tiles - first), t = tile - first * p.m_tiles;
   nt = first + t % wide;
   mt = t / wide;
 }
 
+OGB_DEVICE int i8_cluster_index() {
+  int i;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
+  return i;
+}
 // First k-block of a CTA's range, and the CTA whose range holds one.
 OGB_DEVICE int i8_range_begin(const Int8Params& p, int cta) { return cta * p.range + min(cta, p.longer); }
 OGB_DEVICE int i8_range_owner(const Int8Params& p, int i) {
@@ -90,20 +100,18 @@ OGB_DEVICE int i8_range_owner(const Int8Params& p, int i) {
 }
 
 // The parts of tiles that a CTA computes, in order: of its range the tile it shares with the CTA before it, the one it shares with the CTA
-// after it and the whole ones; then its whole tiles.  (Fewer than 200 tiles of at most 1024 k-blocks are cut: 32 bits hold their sum.)
+// after it and the whole ones; then its whole tiles.  In a cluster one part of one tile, which takes no division: the first loads wait for this.  (Fewer than 200 tiles of at most 1024 k-blocks are cut: 32 bits hold their sum.)
 struct Int8Segs {
   int it0, it1, first_end, last_begin, mid;
   int k_blocks, state = 0, tile, tiles, stride;
   OGB_DEVICE explicit Int8Segs(const Int8Params& p) : k_blocks(p.k_blocks), tiles(p.tiles) {
     stride = gridDim.x;
     if (p.splits > 0) {
-      // one part of one tile, which `mid` finds whole
-      const int t = blockIdx.x / p.splits, rank = blockIdx.x - t * p.splits;
-      it0 = t * k_blocks + k_blocks * rank / p.splits;
-      it1 = t * k_blocks + k_blocks * (rank + 1) / p.splits;
-      first_end = it1;
-      last_begin = mid = it1;
-      tile = tiles;
+      state = 3;
+      tile = p.splits == 1 ? blockIdx.x : i8_cluster_index();
+      const int rank = p.splits == 1 ? 0 : cooperative_groups::this_cluster().block_rank();
+      it0 = i8_range_begin(p, rank);
+      it1 = i8_range_begin(p, rank + 1);
       return;
     }
     tile = p.cut + blockIdx.x;
@@ -119,6 +127,10 @@ struct Int8Segs {
     mid = first_end;
   }
   OGB_DEVICE bool next(int& t, int& kb0, int& kb1) {
+    if (state >= 3) {
+      t = tile; kb0 = it0; kb1 = it1;
+      return state++ == 3;
+    }
     int a = 0, b = 0;
     if (state == 0) { a = it0; b = first_end; state = 1; }
     if (state == 1 && a >= b) { a = last_begin; b = it1; state = 2; }
@@ -444,7 +456,8 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
   bool ok = true;
   pdl_wait();
   const float* factor = after_wait(p.factor);
-  const int tile = blockIdx.x / p.splits, rank = blockIdx.x % p.splits;
+  const int rank = p.splits == 1 ? 0 : cooperative_groups::this_cluster().block_rank();
+  const int tile = p.splits == 1 ? blockIdx.x : i8_cluster_index();
   int nt, mt;
   i8_tile(p, tile, nt, mt);
   const int row0 = mt * p.mn, rows = min(p.mn, p.M - row0);
@@ -476,7 +489,8 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
   }
   if (p.splits > 1) cooperative_groups::this_cluster().sync();
   else __syncthreads();
-  constexpr int kRows = 4 / TW;                     // at a time
+  constexpr int kRows = 2;                   // at a time
+#pragma unroll 1
   for (int m0 = first, k = 0; m0 < rows; m0 += stride * kRows, k += kRows) {
     float s[kRows];
     int4 sum[TW][kRows];
@@ -486,24 +500,34 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
       s[j] = __shfl_sync(0xffffffffu, f, (k + j) & 31);
       if (TW == 1 && p.residual != nullptr && m0 + stride * j < rows) res[j].load(p, ch, row0 + m0 + stride * j);
     }
+    // two CTAs at a time, in a loop: a launch runs this code once or twice, and unrolled it waits for instructions
 #pragma unroll
     for (int w = 0; w < TW; ++w)
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int* src = stage + (w * acc_cols + min(m0 + stride * j, rows - 1)) * 128;
-        if (p.splits == 1) {
-          sum[w][j] = ch.sums(src);
-          continue;
+      for (int j = 0; j < kRows; ++j) sum[w][j] = make_int4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int x = 0; x < p.splits; x += 2) {
+      int4 t[2][TW][kRows];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < TW; ++w)
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            const int* src = stage + (w * acc_cols + min(m0 + stride * j, rows - 1)) * 128;
+            t[i][w][j] = ch.sums(p.splits > 1 ? cooperative_groups::this_cluster().map_shared_rank(src, min(x + i, p.splits - 1)) : src);
+          }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (x + i < p.splits) {
+#pragma unroll
+          for (int w = 0; w < TW; ++w)
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) {
+              sum[w][j].x += t[i][w][j].x; sum[w][j].y += t[i][w][j].y; sum[w][j].z += t[i][w][j].z; sum[w][j].w += t[i][w][j].w;
+            }
         }
-        int4 t[kRowsMaxSplit];
-#pragma unroll
-        for (int x = 0; x < kRowsMaxSplit; ++x)
-          if (x < p.splits) t[x] = ch.sums(cooperative_groups::this_cluster().map_shared_rank(src, x));
-        sum[w][j] = t[0];
-#pragma unroll
-        for (int x = 1; x < kRowsMaxSplit; ++x)
-          if (x < p.splits) { sum[w][j].x += t[x].x; sum[w][j].y += t[x].y; sum[w][j].z += t[x].z; sum[w][j].w += t[x].w; }
-      }
+    }
     i8_store<TW, OUT>(p, ch, row0 + m0, stride, row0 + rows, s, sum[0], sum[TW - 1], res);
   }
   // nobody leaves what is being read
@@ -877,6 +901,8 @@ static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long l
   int grid = ogb_num_sms();
   if (plan.clusters) {
     p.splits = rows_pick_splits(kernel, kI8Threads, smem, p.tiles, p.k_blocks);
+    p.range = p.k_blocks / p.splits;
+    p.longer = p.k_blocks % p.splits;
     grid = p.tiles * p.splits;
   }
   CUtensorMap mw, mq;
