@@ -69,7 +69,7 @@ struct QuantizeParams {
 };
 
 template <int E, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : kMostThreads, WARP ? 12 : V <= kVec ? 2 : 1) quantize_rows_kernel(const QuantizeParams p) {
+__global__ void __launch_bounds__(WARP ? 128 : kMostThreads, WARP ? 12 : (V <= kVec ? 2 : 1) + (E != kElemF32 ? 1 : 0)) quantize_rows_kernel(const QuantizeParams p) {
   __shared__ __align__(16) uint32_t part[kMostThreads / 32];
   pdl_trigger();
   pdl_wait();

@@ -529,3 +529,11 @@ extern "C" int ogb_token_logprobs(const void* logits, const int* tokens, float* 
   if (elem == kElemBf16) return launch_logprobs<__nv_bfloat16>(p, stream);
   return launch_logprobs<__half>(p, stream);
 }
+
+// The same call with its arguments as 64-bit words: see ogb_gemm_int8_args.
+extern "C" int ogb_token_logprobs_args(const int64_t* a) {
+  auto p = [&](int i) { return reinterpret_cast<void*>(a[i]); };
+  auto n = [&](int i) { return static_cast<int>(a[i]); };
+  return ogb_token_logprobs(p(0), static_cast<const int*>(p(1)), static_cast<float*>(p(2)), static_cast<float*>(p(3)), static_cast<int*>(p(4)),
+                            static_cast<int*>(p(5)), static_cast<float*>(p(6)), n(7), n(8), a[9], n(10), n(11), static_cast<int*>(p(12)), p(13));
+}

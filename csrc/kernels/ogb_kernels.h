@@ -286,6 +286,7 @@ int ogb_block_norm_args(const int64_t* args);
 // to 32) with theirs.
 int ogb_token_logprobs(const void* logits, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
                        int rows, int vocab, int64_t ld, int top, int elem, int* status, void* stream);
+int ogb_token_logprobs_args(const int64_t* args);
 
 // MoE: softmax router with top-k (renormalised), device-side permutation by expert, grouped GEMM, combine.
 int ogb_moe_route_topk(const void* router_logits, int* topk_ids, float* topk_w, int tokens, int experts, int k,

@@ -12,6 +12,7 @@ import collections
 import contextlib
 import math
 import os
+import struct
 import threading
 from typing import NamedTuple
 
@@ -560,6 +561,7 @@ class TokenLogprobs(NamedTuple):
 
 _LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TOKEN_TYPES = (torch.int32, torch.int64)
+_pack_logprobs = struct.Struct("14q").pack      # a call with its arguments in one word: ctypes converts them one by one else
 MAX_TOP_LOGPROBS = 32
 MAX_VOCAB, MAX_VOCAB_WITH_TOP = 1 << 30, 3_000_000
 
@@ -605,9 +607,9 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
         # (a matrix by its strides: torch.empty takes twice as long for two dimensions as for one)
         ids = torch.empty_strided((rows, top), (top, 1), dtype=torch.int32, device=dev)
         lps = torch.empty_strided((rows, top), (top, 1), dtype=torch.float32, device=dev)
-    rc = _native.load().ogb_token_logprobs(logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ent.data_ptr() if entropy else 0, rank.data_ptr(),
-                                           ids.data_ptr() if top else 0, lps.data_ptr() if top else 0, rows, vocab, ld, top, kind, status_ptr(index),
-                                           _raw_stream(index))
+    rc = _native.load().ogb_token_logprobs_args(_pack_logprobs(
+        logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), ent.data_ptr() if entropy else 0, rank.data_ptr(), ids.data_ptr() if top else 0,
+        lps.data_ptr() if top else 0, rows, vocab, ld, top, kind, status_ptr(index), _raw_stream(index)))
     _native.check(rc, "ogb_token_logprobs")
     launch_counts["token_logprobs"] += 1
     return TokenLogprobs(logprob, rank, ent, ids, lps)

@@ -51,6 +51,7 @@ _SIGNATURES = {
     "ogb_sample_f32": ([P, P, P, P, P, P, P, P, I, I, I, P], I),
     "ogb_argmax_bf16": ([P, P, I, I, I, P], I),
     "ogb_sample_bf16": ([P, P, P, P, P, P, P, P, I, I, I, P], I),
+    "ogb_token_logprobs_args": ([ctypes.c_char_p], I),
     "ogb_token_logprobs": ([P] * 7 + [I, I, L, I, I, P, P], I),
     "ogb_spec_verify_greedy": ([P, P, P, P, I, I, I, I, P], I),
     "ogb_kv_page_copy": ([P, P, P, I, L, P], I),
