@@ -13,6 +13,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "int8_rows.cuh"
@@ -63,13 +64,60 @@ struct QuantizeParams {
   int8_t* q;
   float* factor;
   long long ldx, ldq;
-  int rows, cols, elem, vec;
+  int rows, cols, elem, shifted;               // shifted: rows do not all begin at multiples of eight values
   unsigned int* counters;
   int num_counters;
 };
 
 template <int E, int V, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : kMostThreads, WARP ? 12 : (V <= kVec ? 2 : 1) + (E != kElemF32 ? 1 : 0)) quantize_rows_kernel(const QuantizeParams p) {
+  __shared__ __align__(16) uint32_t part[kMostThreads / 32];
+  extern __shared__ __align__(16) uint2 exchange[];             // codes of every piece and of one behind them, where rows are shifted
+  pdl_trigger();
+  pdl_wait();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.num_counters; i += blockDim.x) p.counters[i] = 0;
+  const int threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= p.rows) return;
+  const void* x = after_wait(p.x);
+  const size_t at = static_cast<size_t>(row) * p.ldx, to = static_cast<size_t>(row) * p.ldq;
+  const int step = threads * 8, shift = row_shift(row, p.ldx), i0 = tid * 8 - shift;
+  Raw8<E> f[V];
+  uint32_t peak = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v].load(x, at, i0 + v * step, p.cols);
+#pragma unroll
+  for (int v = 0; v < V; ++v) peak = f[v].peak(peak);
+  const RowCode code(row_max<WARP>(Raw8<E>::peak_float(peak), part));
+  if (tid == 0) p.factor[row] = code.factor;
+  uint2 codes[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float t[8];
+    f[v].get(t);
+    codes[v] = E == kElemF32 ? code.codes(t) : code.codes_short(t);
+  }
+  if (p.shifted == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (i0 + v * step < p.cols) store_codes(p.q, to, i0 + v * step, codes[v]);
+    return;
+  }
+  uint2* mine = exchange + (WARP ? (threadIdx.x >> 5) * (32 * V + 1) : 0);
+#pragma unroll
+  for (int v = 0; v < V; ++v) mine[tid + v * threads] = codes[v];
+  if (tid == 0) mine[V * threads] = make_uint2(0, 0);
+  if (WARP) __syncwarp();
+  else __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (tid * 8 + v * step < p.cols) store_codes(p.q, to, tid * 8 + v * step, shift_codes(codes[v], mine[tid + v * threads + 1], shift));
+}
+
+// Rows of any length and alignment.
+template <int V, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : kMostThreads, WARP ? 8 : 2) quantize_any_rows_kernel(const QuantizeParams p) {
   __shared__ __align__(16) uint32_t part[kMostThreads / 32];
   pdl_trigger();
   pdl_wait();
@@ -80,32 +128,26 @@ __global__ void __launch_bounds__(WARP ? 128 : kMostThreads, WARP ? 12 : (V <= k
   if (row >= p.rows) return;
   const void* x = after_wait(p.x);
   const size_t at = static_cast<size_t>(row) * p.ldx, to = static_cast<size_t>(row) * p.ldq;
-  const int step = threads * 8;
-  Raw8<E> f[V];
+  float f[V][8];
   uint32_t peak = 0;
 #pragma unroll
-  for (int v = 0; v < V; ++v) f[v].load(x, p.vec != 0, at, tid * 8 + v * step, p.cols);
+  for (int v = 0; v < V; ++v) load_strided(x, p.elem, at, tid + v * 8 * threads, threads, p.cols, f[v]);
 #pragma unroll
-  for (int v = 0; v < V; ++v) peak = f[v].peak(peak);
+  for (int v = 0; v < V; ++v) peak = max(peak, peak_bits8(f[v]));
   // longer rows than the registers hold are read again below
-  for (int i = tid * 8 + V * step; i < p.cols; i += step) {
-    Raw8<E> t;
-    t.load(x, p.vec != 0, at, i, p.cols);
-    peak = t.peak(peak);
-  }
-  const RowCode code(row_max<WARP>(Raw8<E>::peak_float(peak), part));
-  auto store = [&](const Raw8<E>& r, int i) {
+  for (int i = tid + V * 8 * threads; i < p.cols; i += 8 * threads) {
     float t[8];
-    r.get(t);
-    store_codes(p.q, to, i, E == kElemF32 ? code.codes(t) : code.codes_short(t));
-  };
+    load_strided(x, p.elem, at, i, threads, p.cols, t);
+    peak = max(peak, peak_bits8(t));
+  }
+  const RowCode code(row_max<WARP>(peak, part));
+  auto codes = [&](const float (&t)[8]) { return p.elem == kElemF32 ? code.codes(t) : code.codes_short(t); };
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    if (tid * 8 + v * step < p.cols) store(f[v], tid * 8 + v * step);
-  for (int i = tid * 8 + V * step; i < p.cols; i += step) {
-    Raw8<E> t;
-    t.load(x, p.vec != 0, at, i, p.cols);
-    store(t, i);
+  for (int v = 0; v < V; ++v) store_codes_strided(p.q, to, tid + v * 8 * threads, threads, p.cols, codes(f[v]));
+  for (int i = tid + V * 8 * threads; i < p.cols; i += 8 * threads) {
+    float t[8];
+    load_strided(x, p.elem, at, i, threads, p.cols, t);
+    store_codes_strided(p.q, to, i, threads, p.cols, codes(t));
   }
   if (tid == 0) p.factor[row] = code.factor;
 }
@@ -119,19 +161,28 @@ static int row_threads(int rows, int cols, int most) {
 
 template <int E>
 static int launch_quantize(const QuantizeParams& p, cudaStream_t stream) {
-  int t = row_threads(p.rows, p.cols, kVec);
-  const int pieces = (p.cols + 7) / 8;
+  const int cols = p.cols + (p.shifted != 0 ? 7 : 0), pieces = (cols + 7) / 8;
+  int t = row_threads(p.rows, cols, kVec);
   const bool one = pieces <= t, more = pieces > kVec * t;
-  if (more) t = row_threads(p.rows, p.cols, 2 * kVec);
+  if (more) t = row_threads(p.rows, cols, 2 * kVec);
+  const int v = t == 32 ? (one ? 1 : kVec) : one ? 1 : more ? 2 * kVec : kVec;
   const dim3 grid(t == 32 ? (p.rows + 3) / 4 : p.rows), block(t == 32 ? 128 : t);
+  const int smem = p.shifted != 0 ? 8 * (t == 32 ? 4 * (32 * v + 1) : v * t + 1) : 0;
   auto kernel = t == 32 ? (one ? quantize_rows_kernel<E, 1, true> : quantize_rows_kernel<E, kVec, true>)
                         : (one ? quantize_rows_kernel<E, 1, false> : more ? quantize_rows_kernel<E, 2 * kVec, false> : quantize_rows_kernel<E, kVec, false>);
-  return static_cast<int>(launch_overlapped(kernel, grid, block, 0, stream, p));
+  return static_cast<int>(launch_overlapped(kernel, grid, block, smem, stream, p));
 }
 
 int launch_quantize_rows(const void* x, int8_t* q, float* factor, int rows, int cols, long long ldx, long long ldq, int elem, unsigned int* counters,
                          int num_counters, cudaStream_t stream) {
-  const QuantizeParams p{x, q, factor, ldx, ldq, rows, cols, elem, rows_aligned(x, ldx, elem), counters, num_counters};
+  const QuantizeParams p{x, q, factor, ldx, ldq, rows, cols, elem, ldx % 8 != 0 ? 1 : 0, counters, num_counters};
+  // rows that stay in registers, and a matrix that begins at a multiple of eight values
+  if (!starts_aligned(x, elem) || cols + 7 > 2 * kVec * 8 * kMostThreads) {
+    const int t = row_threads(rows, cols, 2);
+    const dim3 grid(t == 32 ? (rows + 3) / 4 : rows), block(t == 32 ? 128 : t);
+    auto kernel = t == 32 ? quantize_any_rows_kernel<2, true> : (cols <= 8 * t ? quantize_any_rows_kernel<1, false> : quantize_any_rows_kernel<2, false>);
+    return static_cast<int>(launch_overlapped(kernel, grid, block, 0, stream, p));
+  }
   if (elem == kElemF32) return launch_quantize<kElemF32>(p, stream);
   if (elem == kElemBf16) return launch_quantize<kElemBf16>(p, stream);
   return launch_quantize<kElemF16>(p, stream);
@@ -148,157 +199,81 @@ struct BlockNormParams {
   long long ldx, ldy, ldg, ldxo, ldh, ldq;    // ldg 0: one gate for all rows
   int rows, cols;
   int x_elem, y_elem, gate_elem, w_elem, h_elem;
-  int x_vec, y_vec, gate_vec, post_vec, pre_vec, xo_vec, h_vec;
   int gate_sigmoid;
-  int xo_wide;                                 // rows of x_out begin at multiples of 32 bytes
+  int xo_wide, h_wide;                         // 32-byte stores (of 32-bit values)
+  int shifted;                                 // rows do not all begin at multiples of eight values
   int stages;                                  // rows in shared memory: this one and the next, or this one
   float eps, x_scale, y_scale;
-};
-
-// A matrix that rows are read from, through shared memory: a thread fetches what it will use itself, so that a wait for its own copies is all
-// the order there is.
-struct RowSource {
-  const void* p;
-  int elem, vec;
-  long long ld;
-  OGB_DEVICE int words() const { return p == nullptr ? 0 : elem == kElemF32 ? 2 : 1; }        // 16-byte words a piece
-  OGB_DEVICE void fetch(uint4* slot, int threads, int row, int i, int n) const {
-    if (vec == 0 || i + 8 > n) return;
-    const char* s = static_cast<const char*>(p) + (static_cast<size_t>(row) * ld + i) * (elem == kElemF32 ? 4 : 2);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot)), "l"(s) : "memory");
-    if (elem == kElemF32) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot + threads)), "l"(s + 16) : "memory");
-  }
-  OGB_DEVICE void get(const uint4* slot, int threads, int row, int i, int n, float (&f)[8]) const {
-    if (vec == 0 || i + 8 > n) {           // unaligned rows, and what a row's end leaves of a piece
-      load8(p, elem, false, static_cast<size_t>(row) * ld, i, n, f);
-      return;
-    }
-    const uint4 a = slot[0];
-    if (elem == kElemF32) {
-      const uint4 b = slot[threads];
-      const Raw8<kElemF32> r{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-      r.get(f);
-    } else if (elem == kElemBf16) {
-      const Raw8<kElemBf16> r{{a.x, a.y, a.z, a.w}};
-      r.get(f);
-    } else {
-      const Raw8<kElemF16> r{{a.x, a.y, a.z, a.w}};
-      r.get(f);
-    }
-  }
 };
 
 // Blocks an SM holds at least, which bounds the registers: 80 a thread with four pieces, 64 with fewer.
 constexpr int norm_blocks(int v, int t) { return 65536 / ((v < kVec ? 64 : 80) * (t == 32 ? 128 : t)); }
 
-// T: most threads of a block, 32: a warp a row.
+// Any types, sizes and alignments.  T: most threads of a block, 32: a warp a row.
 template <int V, int T>
-__global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_norm_kernel(const BlockNormParams p) {
+__global__ void __launch_bounds__(T == 32 ? 128 : T, V < kVec ? norm_blocks(V, T) : 1) block_norm_kernel(const BlockNormParams p) {
   __shared__ __align__(16) float part_y[2][kMostThreads / 32], part_x[2][kMostThreads / 32];
   __shared__ __align__(16) uint32_t part_q[2][kMostThreads / 32];
-  extern __shared__ __align__(16) uint4 slots[];
   constexpr bool WARP = T == 32;
+  constexpr int N = 8 * V;
   pdl_trigger();
   pdl_wait();
-  const int threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int step = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int warps = WARP ? blockDim.x >> 5 : 1, rows_step = gridDim.x * warps;
-  const int n = p.cols, step = threads * 8, i0 = tid * 8, all = blockDim.x;
+  const int n = p.cols;
   const float over = 1.f / static_cast<float>(n);
-  const RowSource xs{after_wait(p.x), p.x_elem, p.x_vec, p.ldx};
-  const RowSource ys{after_wait(p.y), p.y_elem, p.y_vec, p.ldy};
-  const bool gate_row = p.gate != nullptr && p.ldg != 0;                      // a gate for all rows stays in cache
-  const RowSource gs{gate_row ? after_wait(p.gate) : nullptr, p.gate_elem, p.gate_vec, p.ldg};
-  const int wx = xs.words(), wy = ys.words(), wg = gs.words(), words = V * (wx + wy + wg);
-  uint4* mine = slots + threadIdx.x;                                          // word w of a stage: mine[w * all]
-  auto fetch = [&](int row, int stage) {
-    uint4* to = mine + stage * words * all;
+  const void *xp = after_wait(p.x), *yp = after_wait(p.y), *gp = after_wait(p.gate);
+  int turn = 0;
+  for (int row = blockIdx.x * warps + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += rows_step, turn ^= 1) {
+    float x[N], t[N];
+    load_strided(xp, p.x_elem, static_cast<size_t>(row) * p.ldx, tid, step, n, x);
+    if (yp != nullptr) {
+      float y[N], ry = p.y_scale, sum = 0.f;
+      load_strided(yp, p.y_elem, static_cast<size_t>(row) * p.ldy, tid, step, n, y);
+      if (gp != nullptr) load_strided(gp, p.gate_elem, static_cast<size_t>(row) * p.ldg, tid, step, n, t);
+      if (p.post != nullptr) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = i0 + v * step;
-      xs.fetch(to + v * wx * all, all, row, i, n);
-      if (wy != 0) ys.fetch(to + (V * wx + v * wy) * all, all, row, i, n);
-      if (wg != 0) gs.fetch(to + (V * (wx + wy) + v * wg) * all, all, row, i, n);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  int row = blockIdx.x * warps + (WARP ? threadIdx.x >> 5 : 0);
-  if (p.stages == 2 && row < p.rows) fetch(row, 0);
-  for (int turn = 0; row < p.rows; row += rows_step, turn ^= 1) {
-    if (p.stages == 1) fetch(row, 0);
-    else if (row + rows_step < p.rows) fetch(row + rows_step, turn ^ 1);
-    if (p.stages == 2 && row + rows_step < p.rows) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const uint4* from = mine + (p.stages == 2 ? turn * words * all : 0);
-    float ry = p.y_scale;
-    if (p.post != nullptr) {
-      float sum = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float y[8];
-        ys.get(from + (V * wx + v * wy) * all, all, row, i0 + v * step, n, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(y[j], y[j], sum);
+        for (int j = 0; j < N; ++j) sum = fmaf(y[j], y[j], sum);
       }
-      ry *= rsqrtf(row_sum<WARP>(sum, part_y[turn]) * over + p.eps);
-    }
-    float x[V][8], sum = 0.f;
+      if (gp != nullptr) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int i = i0 + v * step;
-      xs.get(from + v * wx * all, all, row, i, n, x[v]);
-      if (wy != 0) {
-        float y[8], t[8];
-        ys.get(from + (V * wx + v * wy) * all, all, row, i, n, y);
-        if (p.post != nullptr) {
-          load8(p.post, p.w_elem, p.post_vec != 0, 0, i, n, t);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] *= t[j];
-        }
-        if (p.gate != nullptr) {
-          if (wg != 0) gs.get(from + (V * (wx + wy) + v * wg) * all, all, row, i, n, t);
-          else load8(p.gate, p.gate_elem, p.gate_vec != 0, 0, i, n, t);
-          if (p.gate_sigmoid != 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = __fdividef(y[j], 1.f + __expf(-t[j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= t[j];
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] = fmaf(ry, y[j], p.x_scale * x[v][j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] *= p.x_scale;
+        for (int j = 0; j < N; ++j) y[j] *= p.gate_sigmoid != 0 ? __fdividef(1.f, 1.f + __expf(-t[j])) : t[j];
       }
-      if (p.x_out != nullptr) store8(p.x_out, p.x_elem, p.xo_vec != 0, static_cast<size_t>(row) * p.ldxo, i, n, x[v]);
+      if (p.post != nullptr) {
+        load_strided(p.post, p.w_elem, 0, tid, step, n, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[v][j], x[v][j], sum);      // past the row's end: zeros
+        for (int j = 0; j < N; ++j) y[j] *= t[j];
+        ry *= rsqrtf(row_sum<WARP>(sum, part_y[turn]) * over + p.eps);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = fmaf(ry, y[j], p.x_scale * x[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] *= p.x_scale;
     }
+    if (p.x_out != nullptr) store_strided(p.x_out, p.x_elem, static_cast<size_t>(row) * p.ldxo, tid, step, n, x);
     if (p.h == nullptr && p.q == nullptr) continue;
     if (p.pre != nullptr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) sum = fmaf(x[j], x[j], sum);      // past the row's end: zeros
+      load_strided(p.pre, p.w_elem, 0, tid, step, n, t);
       const float rx = rsqrtf(row_sum<WARP>(sum, part_x[turn]) * over + p.eps);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float t[8];
-        load8(p.pre, p.w_elem, p.pre_vec != 0, 0, i0 + v * step, n, t);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] *= rx * t[j];
-      }
+      for (int j = 0; j < N; ++j) x[j] *= rx * t[j];
     }
-    if (p.h != nullptr) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) store8(p.h, p.h_elem, p.h_vec != 0, static_cast<size_t>(row) * p.ldh, i0 + v * step, n, x[v]);
-    }
+    if (p.h != nullptr) store_strided(p.h, p.h_elem, static_cast<size_t>(row) * p.ldh, tid, step, n, x);
     if (p.q != nullptr) {
       uint32_t peak = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) peak = max(peak, peak_bits8(x[v]));
+      for (int j = 0; j < N; ++j) peak = max(peak, __float_as_uint(x[j]) & 0x7fffffffu);
       const RowCode code(row_max<WARP>(peak, part_q[turn]));
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int i = i0 + v * step;
-        if (i < n) store_codes(p.q, static_cast<size_t>(row) * p.ldq, i, code.codes(x[v]));
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = x[8 * v + j];
+        store_codes_strided(p.q, static_cast<size_t>(row) * p.ldq, tid + v * 8 * step, step, n, code.codes(f));
       }
       if (tid == 0) p.factor[row] = code.factor;
     }
@@ -319,64 +294,116 @@ OGB_DEVICE float sigmoid_approx(float g) {
   return r;
 }
 
-// The same for the usual types and layouts: rows and weights at multiples of 16 bytes, cols a multiple of eight, a stream of type XE, bf16 from the
-// block and to the next one (or 8-bit rows), weights and a gate a channel of type WE.  Weights meet the values before the sum over the row is known,
-// so that what follows a sum is one product; the largest |h| is the largest |x' pre| times the root, so it joins the second sum's exchange.
-template <int XE, int WE, int V, int T>
+// Eight weights from column i on, wherever that is.
+OGB_DEVICE void load_weights(const void* p, int elem, int i, int n, float (&t)[8]) {
+  if ((i & 7) != 0) {                                                          // rows that are shifted against them
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = i + j >= 0 && i + j < n ? load_elem(p, elem, i + j) : 0.f;
+  } else if (elem == kElemF32) {
+    Raw8<kElemF32> w;
+    w.load(p, 0, i, n);
+    w.get(t);
+  } else if (elem == kElemBf16) {
+    Raw8<kElemBf16> w;
+    w.load(p, 0, i, n);
+    w.get(t);
+  } else {
+    Raw8<kElemF16> w;
+    w.load(p, 0, i, n);
+    w.get(t);
+  }
+}
+// Eight results from column i on, one by one at the ends of a row.
+template <int E>
+OGB_DEVICE void store_piece(void* p, size_t row, int i, int n, bool wide, const float (&f)[8]) {
+  if (i >= 0 && i + 8 <= n) {
+    if (E == kElemF32 && wide) store32(static_cast<float*>(p) + row + i, f);
+    else store8(p, E, true, row, i, n, f);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (i + j >= 0 && i + j < n) store_elem(p, E, row + i + j, f[j]);
+}
+
+// The same for matrices that begin at multiples of eight values and share a row stride modulo eight (contiguous ones do): every row is taken in pieces of
+// eight values that lie at such multiples in all of them.  XE: type of the stream, YE: of the block's output, a gate a token and h.  Weights meet the values
+// before the sum over the row is known, so that what follows a sum is one product; the largest |h| is the largest |x' pre| times the root, so it joins the
+// second sum's exchange.  The row comes through shared memory, and the next one with it where there is room.
+template <int XE, int YE, int V, int T>
 __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_norm_usual_kernel(const BlockNormParams p) {
   __shared__ __align__(16) float part_y[2][kMostThreads / 32], part_x[2][kMostThreads / 32];
   __shared__ __align__(16) uint32_t part_q[2][kMostThreads / 32];
   extern __shared__ __align__(16) uint4 slots[];
   constexpr bool WARP = T == 32;
-  constexpr int kX = XE == kElemF32 ? 2 : 1;                                  // 16-byte words of a piece of the stream
+  constexpr int kX = XE == kElemF32 ? 2 : 1, kY = YE == kElemF32 ? 2 : 1;     // 16-byte words of a piece
+  constexpr int kXBytes = XE == kElemF32 ? 4 : 2, kYBytes = YE == kElemF32 ? 4 : 2;
   pdl_trigger();
   pdl_wait();
-  const int threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int threads = WARP ? 32 : blockDim.x, tid = WARP ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31;
   const int warps = WARP ? blockDim.x >> 5 : 1, rows_step = gridDim.x * warps;
-  const int n = p.cols, step = threads * 8, i0 = tid * 8, all = blockDim.x;
+  const int n = p.cols, step = threads * 8, all = blockDim.x;
   const float over = 1.f / static_cast<float>(n);
   const char *x = static_cast<const char*>(after_wait(p.x)), *y = static_cast<const char*>(after_wait(p.y)), *g = static_cast<const char*>(after_wait(p.gate));
   const bool has_y = y != nullptr, gate_row = g != nullptr && p.ldg != 0;
-  const int words = V * (kX + (has_y ? 1 : 0) + (gate_row ? 1 : 0));
-  uint4* mine = slots + threadIdx.x;
+  const int words = V * (kX + (has_y ? kY : 0) + (gate_row ? kY : 0));
+  uint4* mine = slots + threadIdx.x - lane;                                    // the warp's words
   const uint32_t base = smem_u32(mine);
   auto copy = [](uint32_t to, const char* s) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(s) : "memory"); };
-  auto fetch = [&](int row, int stage) {
-    uint32_t to = base + stage * words * all * 16;
+  // A warp's 32 pieces of a matrix: 32 words, or of 32-bit values 64.  Lanes copy neighbouring words, so that no 32-byte sector is asked for twice, and
+  // take two each from shared memory, where words trade places in every other eight to keep eight lanes on different banks.
+  auto fetch_matrix = [&](auto bytes, uint32_t to, const char* s, size_t at, int shift) {
+    constexpr int kBytes = decltype(bytes)::value, kW = kBytes / 2;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (i0 + v * step < n) {
-        if (kX == 1) copy(to + v * all * 16, x + (static_cast<size_t>(row) * p.ldx + i0 + v * step) * 2);
-        if (has_y) copy(to + (V * kX + v) * all * 16, y + (static_cast<size_t>(row) * p.ldy + i0 + v * step) * 2);
-        if (gate_row) copy(to + (V * (kX + 1) + v) * all * 16, g + (static_cast<size_t>(row) * p.ldg + i0 + v * step) * 2);
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int h = 0; h < kW; ++h) {
+        const int w = lane + 32 * h, piece = (tid - lane) * 8 + v * step - shift + 8 * (w / kW);
+        if (piece >= 0 && piece + 8 <= n)
+          copy(to + (v * kW * all + (kW == 2 ? w ^ (w >> 3 & 1) : w)) * 16, s + (at + piece) * kBytes + (w % kW) * 16);
       }
-    }
-    if (kX == 2) {
-      // A warp's 32 pieces are 64 words.  Lanes copy neighbouring ones, so that no 32-byte sector is asked for twice, and take two each from shared
-      // memory, where words trade places in every other eight to keep eight lanes on different banks.
-      const int lane = threadIdx.x & 31;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int w = lane + 32 * h, i = (i0 - 8 * lane) + v * step + 4 * w;
-          if (i < n)
-            copy(base - lane * 16 + (stage * words * all + v * 2 * all + (threadIdx.x - lane) + (w ^ (w >> 3 & 1))) * 16,
-                 x + (static_cast<size_t>(row) * p.ldx + i) * 4);
-        }
-    }
+  };
+  using XBytes = std::integral_constant<int, kXBytes>;
+  using YBytes = std::integral_constant<int, kYBytes>;
+  auto fetch = [&](int row, int stage) {
+    const int shift = row_shift(row, p.ldx);
+    const uint32_t to = base + stage * words * all * 16;
+    // (a warp's 64 words lie next to one another, a block's two sets of 32 a thread apart: every warp's begin at twice its first thread's)
+    fetch_matrix(XBytes(), to + (kX == 2 ? (threadIdx.x - lane) * 16 : 0), x, static_cast<size_t>(row) * p.ldx, shift);
+    if (has_y) fetch_matrix(YBytes(), to + V * kX * all * 16 + (kY == 2 ? (threadIdx.x - lane) * 16 : 0), y, static_cast<size_t>(row) * p.ldy, shift);
+    if (gate_row) fetch_matrix(YBytes(), to + V * (kX + kY) * all * 16 + (kY == 2 ? (threadIdx.x - lane) * 16 : 0), g, static_cast<size_t>(row) * p.ldg, shift);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // piece v of a matrix whose words begin at `from` of this warp's
+  auto get = [&](auto elem, const uint4* from, int v, const char* s, size_t at, int i, float (&t)[8]) {
+    constexpr int E = decltype(elem)::value;
+    Raw8<E> r;
+    if (i < 0 || i + 8 > n) {
+      r.edge(s, at, i, n);
+    } else if constexpr (E == kElemF32) {
+      const uint4* two = from + (threadIdx.x - lane) + v * 2 * all + 2 * lane;
+      const int swap = lane >> 2 & 1;
+      const uint4 lo = two[swap], hi = two[swap ^ 1];
+      r = Raw8<E>{{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}};
+    } else {
+      const uint4 raw = from[v * all + lane];
+      r = Raw8<E>{{raw.x, raw.y, raw.z, raw.w}};
+    }
+    r.get(t);
+  };
+  using XElem = std::integral_constant<int, XE>;
+  using YElem = std::integral_constant<int, YE>;
   int row = blockIdx.x * warps + (WARP ? threadIdx.x >> 5 : 0);
   if (p.stages == 2 && row < p.rows) fetch(row, 0);
   for (int turn = 0; row < p.rows; row += rows_step, turn ^= 1) {
-    if (kX == 2) __syncwarp();                                                // what the copies overwrite has been read by the whole warp
+    __syncwarp();                                                             // what the copies overwrite has been read by the whole warp
     if (p.stages == 1) fetch(row, 0);
     else if (row + rows_step < p.rows) fetch(row + rows_step, turn ^ 1);
     if (p.stages == 2 && row + rows_step < p.rows) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (kX == 2) __syncwarp();
+    __syncwarp();
     const uint4* from = mine + (p.stages == 2 ? turn * words * all : 0);
+    const int i0 = tid * 8 - row_shift(row, p.ldx);
     float a[V][8], ry = p.y_scale;
     if (has_y) {
       float sum = 0.f;
@@ -384,28 +411,19 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
       for (int v = 0; v < V; ++v) {
         const int i = i0 + v * step;
         if (i < n) {
-          const uint4 raw = from[(V * kX + v) * all];
-          Raw8<kElemBf16>{{raw.x, raw.y, raw.z, raw.w}}.get(a[v]);
           float t[8];
+          get(YElem(), from + V * kX * all, v, y, static_cast<size_t>(row) * p.ldy, i, a[v]);
           if (p.post != nullptr) {
-            Raw8<WE> w;
-            w.load(p.post, true, 0, i, n);
-            w.get(t);
+            load_weights(p.post, p.w_elem, i, n, t);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               sum = fmaf(a[v][j], a[v][j], sum);
               a[v][j] *= t[j];
             }
           }
-          if (gate_row) {
-            const uint4 graw = from[(V * (kX + 1) + v) * all];
-            Raw8<kElemBf16>{{graw.x, graw.y, graw.z, graw.w}}.get(t);
-          } else if (g != nullptr) {
-            Raw8<WE> w;
-            w.load(g, true, 0, i, n);
-            w.get(t);
-          }
           if (g != nullptr) {
+            if (gate_row) get(YElem(), from + V * (kX + kY) * all, v, g, static_cast<size_t>(row) * p.ldg, i, t);
+            else load_weights(g, p.gate_elem, i, n, t);
             if (p.gate_sigmoid != 0) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) t[j] = sigmoid_approx(t[j]);
@@ -424,31 +442,16 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
       const int i = i0 + v * step;
       if (i < n) {
         float t[8];
-        if constexpr (kX == 2) {
-          const int lane = threadIdx.x & 31, swap = lane >> 2 & 1;
-          const uint4* two = from - lane + v * 2 * all + (threadIdx.x - lane) + 2 * lane;
-          const uint4 lo = two[swap], hi = two[swap ^ 1];
-          Raw8<kElemF32>{{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}}.get(t);
-        } else {
-          const uint4 raw = from[v * all];
-          Raw8<kElemBf16>{{raw.x, raw.y, raw.z, raw.w}}.get(t);
-        }
+        get(XElem(), from, v, x, static_cast<size_t>(row) * p.ldx, i, t);      // zeros in front of a row and past its end, and so is x'
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           t[j] *= p.x_scale;
           if (has_y) t[j] = fmaf(ry, a[v][j], t[j]);
           a[v][j] = t[j];
         }
-        if (p.x_out != nullptr) {
-          if (XE == kElemF32 && p.xo_wide != 0)
-            store32(static_cast<float*>(p.x_out) + static_cast<size_t>(row) * p.ldxo + i, a[v]);
-          else
-            store8(p.x_out, XE, true, static_cast<size_t>(row) * p.ldxo, i, n, a[v]);
-        }
+        if (p.x_out != nullptr) store_piece<XE>(p.x_out, static_cast<size_t>(row) * p.ldxo, i, n, p.xo_wide != 0, a[v]);
         if (p.pre != nullptr) {
-          Raw8<WE> w;
-          w.load(p.pre, true, 0, i, n);
-          w.get(t);
+          load_weights(p.pre, p.w_elem, i, n, t);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             sum = fmaf(a[v][j], a[v][j], sum);
@@ -463,35 +466,52 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
     if (p.q != nullptr) {
       // both at one exchange
       peak = __reduce_max_sync(0xffffffffu, peak);
-      if (!WARP && (threadIdx.x & 31) == 0) part_q[turn][threadIdx.x >> 5] = peak;
+      if (!WARP && lane == 0) part_q[turn][threadIdx.x >> 5] = peak;
     }
     if (p.pre != nullptr) rx = rsqrtf(row_sum<WARP>(sum, part_x[turn]) * over + p.eps);
     else if (!WARP && p.q != nullptr) __syncthreads();
-    if (p.q != nullptr) {
-      if (!WARP)
-        for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) peak = max(peak, part_q[turn][w]);
-      // infinities and NaN stay above all values; a root that is not a number makes the row one
-      const RowCode code(__float_as_uint(__uint_as_float(peak) * rx) & 0x7fffffffu);
+    if (p.q == nullptr) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = i0 + v * step;
         if (i < n) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) a[v][j] *= rx;
-          store_codes(p.q, static_cast<size_t>(row) * p.ldq, i, code.codes(a[v]));
+          store_piece<YE>(p.h, static_cast<size_t>(row) * p.ldh, i, n, p.h_wide != 0, a[v]);
         }
       }
-      if (tid == 0) p.factor[row] = code.factor;
-    } else {
+      continue;
+    }
+    if (!WARP)
+      for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) peak = max(peak, part_q[turn][w]);
+    // infinities and NaN stay above all values; a root that is not a number makes the row one
+    const RowCode code(__float_as_uint(__uint_as_float(peak) * rx) & 0x7fffffffu);
+    if (tid == 0) p.factor[row] = code.factor;
+    uint2 codes[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int i = i0 + v * step;
-        if (i < n) {
+    for (int v = 0; v < V; ++v) {
+      codes[v] = make_uint2(0, 0);
+      if (i0 + v * step < n) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a[v][j] *= rx;
-          store8(p.h, kElemBf16, true, static_cast<size_t>(row) * p.ldh, i, n, a[v]);
-        }
+        for (int j = 0; j < 8; ++j) a[v][j] *= rx;
+        codes[v] = code.codes(a[v]);
+        if (p.shifted == 0) store_codes(p.q, static_cast<size_t>(row) * p.ldq, i0 + v * step, codes[v]);
       }
+    }
+    if (p.shifted != 0) {
+      // a word of q is made of two pieces: the next one is the next thread's
+      uint2* exchange = reinterpret_cast<uint2*>(slots + p.stages * words * all) + (WARP ? (threadIdx.x >> 5) * (32 * V + 1) : 0);
+      if (WARP) __syncwarp();
+      else __syncthreads();                                                   // of the row before
+#pragma unroll
+      for (int v = 0; v < V; ++v) exchange[tid + v * threads] = codes[v];
+      if (tid == 0) exchange[V * threads] = make_uint2(0, 0);
+      if (WARP) __syncwarp();
+      else __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (tid * 8 + v * step < n)
+          store_codes(p.q, static_cast<size_t>(row) * p.ldq, tid * 8 + v * step, shift_codes(codes[v], exchange[tid + v * threads + 1], row_shift(row, p.ldx)));
     }
   }
 }
@@ -508,25 +528,53 @@ static int launch_norm_kernel(OncePerDevice& allowed, Kernel kernel, BlockNormPa
   // better (8192 rows of 3584, stream in 32 bits with a gate a token: 106 us with three blocks of two rows, 92 with four of one).
   const int most = std::max(1, 65536 / ((V < kVec ? 64 : 80) * block));
   p.stages = (2 * stage + 1024) * most <= kNormSmem ? 2 : 1;
-  const int smem = p.stages * stage;
+  const int exchange = p.q != nullptr && p.shifted != 0 ? (8 * (T == 32 ? 4 * (32 * V + 1) : V * block + 1) + 15) / 16 * 16 : 0;
+  const int smem = p.stages * stage + exchange;
   const int per_sm = std::max(1, std::min(kNormSmem / (smem + 1024), most));
   const int grid = std::min(T == 32 ? (p.rows + 3) / 4 : p.rows, ogb_num_sms() * per_sm);
   return static_cast<int>(launch_overlapped(kernel, dim3(grid), dim3(block), smem, stream, p));
 }
 template <int V, int T>
-static int launch_norm(const BlockNormParams& p, int threads, cudaStream_t stream) {
-  static OncePerDevice allowed[5];
-  const bool aligned = p.x_vec != 0 && p.y_vec != 0 && p.gate_vec != 0 && p.post_vec != 0 && p.pre_vec != 0 && p.xo_vec != 0 && p.h_vec != 0;
-  const bool bf16 = (p.y == nullptr || p.y_elem == kElemBf16) && (p.gate == nullptr || p.gate_elem == (p.ldg != 0 ? kElemBf16 : p.w_elem)) &&
-                    (p.h == nullptr || p.h_elem == kElemBf16) && (p.h == nullptr || p.q == nullptr);
-  if (aligned && bf16 && p.cols % 8 == 0 && p.x_elem != kElemF16 && p.w_elem != kElemF16) {
-    if (p.x_elem == kElemF32)
-      return p.w_elem == kElemF32 ? launch_norm_kernel<V, T>(allowed[0], block_norm_usual_kernel<kElemF32, kElemF32, V, T>, p, threads, stream)
-                                  : launch_norm_kernel<V, T>(allowed[1], block_norm_usual_kernel<kElemF32, kElemBf16, V, T>, p, threads, stream);
-    return p.w_elem == kElemF32 ? launch_norm_kernel<V, T>(allowed[2], block_norm_usual_kernel<kElemBf16, kElemF32, V, T>, p, threads, stream)
-                                : launch_norm_kernel<V, T>(allowed[3], block_norm_usual_kernel<kElemBf16, kElemBf16, V, T>, p, threads, stream);
+static int launch_usual(const BlockNormParams& p, int threads, cudaStream_t stream) {
+  static OncePerDevice allowed[6];
+#define OGB_NORM(AT, XE, YE) return launch_norm_kernel<V, T>(allowed[AT], block_norm_usual_kernel<XE, YE, V, T>, p, threads, stream)
+  if (p.x_elem == kElemF32) {
+    if (p.y_elem == kElemF32) OGB_NORM(0, kElemF32, kElemF32);
+    if (p.y_elem == kElemBf16) OGB_NORM(1, kElemF32, kElemBf16);
+    OGB_NORM(2, kElemF32, kElemF16);
   }
-  return launch_norm_kernel<V, T>(allowed[4], block_norm_kernel<V, T>, p, threads, stream);
+  if (p.y_elem == kElemF32) OGB_NORM(3, kElemBf16, kElemF32);
+  if (p.y_elem == kElemBf16) OGB_NORM(4, kElemBf16, kElemBf16);
+  OGB_NORM(5, kElemBf16, kElemF16);
+#undef OGB_NORM
+}
+template <int V, int T>
+static int launch_any(const BlockNormParams& p, int threads, cudaStream_t stream) {
+  const int block = T == 32 ? 128 : threads;
+  const int per_sm = V < kVec ? std::max(1, 65536 / (64 * block)) : std::max(1, 65536 / (128 * block));
+  const int grid = std::min(T == 32 ? (p.rows + 3) / 4 : p.rows, ogb_num_sms() * per_sm);
+  return static_cast<int>(launch_overlapped(block_norm_kernel<V, T>, dim3(grid), dim3(block), 0, stream, p));
+}
+static int launch_norm(BlockNormParams p, cudaStream_t stream) {
+  // a type for the block's side of it: of what there is of its output, a gate a token and h
+  int side = p.y != nullptr ? p.y_elem : p.h != nullptr ? p.h_elem : kElemBf16;
+  auto goes = [&](const void* m, long long ld, int elem, int type) { return m == nullptr || (elem == type && starts_aligned(m, elem) && (ld - p.ldx) % 8 == 0); };
+  auto vector = [](const void* m) { return (reinterpret_cast<uintptr_t>(m) & 15) == 0; };
+  const bool usual = p.x_elem != kElemF16 && goes(p.x, p.ldx, p.x_elem, p.x_elem) && goes(p.x_out, p.ldxo, p.x_elem, p.x_elem) && goes(p.y, p.ldy, p.y_elem, side) &&
+                     goes(p.h, p.ldh, p.h_elem, side) && (p.gate == nullptr || p.ldg == 0 || goes(p.gate, p.ldg, p.gate_elem, side)) && vector(p.post) &&
+                     vector(p.pre) && (p.ldg != 0 || vector(p.gate)) && !(p.h != nullptr && p.q != nullptr) && p.cols + 7 <= kNormMaxCols;
+  if (!usual) {
+    const int t = row_threads(p.rows, p.cols, 2), pieces = (p.cols + 7) / 8;
+    if (t == 32) return launch_any<2, 32>(p, t, stream);
+    if (pieces <= t) return launch_any<1, kMostThreads>(p, t, stream);
+    return pieces <= 2 * t ? launch_any<2, kMostThreads>(p, t, stream) : launch_any<kVec, kMostThreads>(p, t, stream);
+  }
+  p.y_elem = side;
+  p.shifted = p.ldx % 8 != 0 ? 1 : 0;
+  const int cols = p.cols + (p.shifted != 0 ? 7 : 0), t = row_threads(p.rows, cols, 2), pieces = (cols + 7) / 8;
+  if (t == 32) return launch_usual<2, 32>(p, t, stream);
+  if (pieces <= t) return launch_usual<1, kMostThreads>(p, t, stream);
+  return pieces <= 2 * t ? launch_usual<2, kMostThreads>(p, t, stream) : launch_usual<kVec, kMostThreads>(p, t, stream);
 }
 
 }  // namespace ogb
@@ -549,15 +597,9 @@ extern "C" int ogb_block_norm(const void* x, const void* y, const void* gate, co
   if (rows < 0 || cols < 1 || cols > kNormMaxCols) return -2;
   if (rows == 0) return 0;
   if (q != nullptr && (ldq < cols || (ldq & 15) != 0 || (reinterpret_cast<uintptr_t>(q) & 15) != 0 || factor == nullptr)) return -3;
-  BlockNormParams p{x, y, gate, post, pre, x_out, h, static_cast<int8_t*>(q), factor, ldx, ldy, ldg, ldxo, ldh, ldq, rows, cols, x_elem, y_elem, gate_elem,
-                    w_elem, h_elem, rows_aligned(x, ldx, x_elem), rows_aligned(y, ldy, y_elem), rows_aligned(gate, ldg, gate_elem),
-                    rows_aligned(post, 0, w_elem), rows_aligned(pre, 0, w_elem), rows_aligned(x_out, ldxo, x_elem), rows_aligned(h, ldh, h_elem),
-                    gate_sigmoid, (reinterpret_cast<uintptr_t>(x_out) & 31) == 0 && ldxo % 8 == 0 ? 1 : 0, 2, eps, x_scale, y_scale};
-  const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const int t = row_threads(rows, cols, 2), pieces = (cols + 7) / 8;
-  if (t == 32) return launch_norm<2, 32>(p, t, stream);
-  if (pieces <= t) return launch_norm<1, kMostThreads>(p, t, stream);
-  return pieces <= 2 * t ? launch_norm<2, kMostThreads>(p, t, stream) : launch_norm<kVec, kMostThreads>(p, t, stream);
+  const BlockNormParams p{x, y, gate, post, pre, x_out, h, static_cast<int8_t*>(q), factor, ldx, ldy, ldg, ldxo, ldh, ldq, rows, cols, x_elem, y_elem, gate_elem,
+                          w_elem, h_elem, gate_sigmoid, 1, 1, 0, 2, eps, x_scale, y_scale};
+  return launch_norm(p, static_cast<cudaStream_t>(stream_));
 }
 
 // The same call with its arguments as 64-bit words, floating ones as doubles: see ogb_gemm_int8_args.

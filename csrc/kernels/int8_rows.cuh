@@ -15,6 +15,10 @@ inline int elem_bytes(int elem) { return elem == kElemF32 ? 4 : 2; }
 inline int rows_aligned(const void* p, long long ld, int elem) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * elem_bytes(elem) & 15) == 0 ? 1 : 0;
 }
+// A matrix begins at a multiple of eight values.  Its rows then begin (row * ld) mod 8 values past one, and are taken in pieces of eight that lie at
+// such multiples, the first of them so many values in front of the row.
+inline bool starts_aligned(const void* p, int elem) { return (reinterpret_cast<uintptr_t>(p) & (8 * elem_bytes(elem) - 1)) == 0; }
+OGB_DEVICE int row_shift(int row, long long ld) { return static_cast<int>((static_cast<unsigned>(row) * static_cast<unsigned>(ld & 7)) & 7u); }
 
 OGB_DEVICE float load_elem(const void* p, int elem, size_t at) {
   if (elem == kElemF32) return static_cast<const float*>(p)[at];
@@ -72,14 +76,52 @@ OGB_DEVICE void store8(void* p, int elem, bool vec, size_t row, int i, int n, co
     if (i + j < n) store_elem(p, elem, row + i + j, f[j]);
 }
 
+// Where rows do not begin at multiples of 16 bytes a thread takes every `step`-th value instead of neighbours, so that a warp's accesses still meet
+// whole sectors.  N values from column i on of a row that begins at value `row` and has n; zeros past its end.
+template <int N>
+OGB_DEVICE void load_strided(const void* p, int elem, size_t row, int i, int step, int n, float (&f)[N]) {
+  if (elem == kElemF32) {
+    const float* s = static_cast<const float*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = i + j * step < n ? s[i + j * step] : 0.f;
+  } else if (elem == kElemBf16) {
+    const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = i + j * step < n ? __bfloat162float(s[i + j * step]) : 0.f;
+  } else {
+    const __half* s = static_cast<const __half*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = i + j * step < n ? __half2float(s[i + j * step]) : 0.f;
+  }
+}
+template <int N>
+OGB_DEVICE void store_strided(void* p, int elem, size_t row, int i, int step, int n, const float (&f)[N]) {
+  if (elem == kElemF32) {
+    float* d = static_cast<float*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j * step < n) d[i + j * step] = f[j];
+  } else if (elem == kElemBf16) {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j * step < n) d[i + j * step] = __float2bfloat16(f[j]);
+  } else {
+    __half* d = static_cast<__half*>(p) + row;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j * step < n) d[i + j * step] = __float2half_rn(f[j]);
+  }
+}
+
 // Eight neighbouring values as they lie in memory.
 template <int E>
 struct Raw8 {
   static constexpr int kWords = E == kElemF32 ? 8 : 4;
   uint32_t w[kWords];
-  // from column i on of a row that begins at value `row` and has n; zeros past its end
-  OGB_DEVICE void load(const void* p, bool vec, size_t row, int i, int n) {
-    if (vec && i + 8 <= n) {
+  // from column i on of a row that begins at value `row` and has n, at a multiple of eight values; zeros in front of it and past its end
+  OGB_DEVICE void load(const void* p, size_t row, int i, int n) {
+    if (i >= 0 && i + 8 <= n) {
       const uint4* s = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + (row + i) * (E == kElemF32 ? 4 : 2));
       const uint4 a = s[0];
       w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
@@ -89,14 +131,17 @@ struct Raw8 {
       }
       return;
     }
+    edge(p, row, i, n);
+  }
+  OGB_DEVICE void edge(const void* p, size_t row, int i, int n) {
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      if constexpr (E == kElemF32) {
-        w[j] = i + j < n ? static_cast<const uint32_t*>(p)[row + i + j] : 0;
-      } else {
-        const uint16_t* s = static_cast<const uint16_t*>(p) + row + i + 2 * j;
-        w[j] = (i + 2 * j < n ? s[0] : 0u) | (i + 2 * j + 1 < n ? static_cast<uint32_t>(s[1]) << 16 : 0u);
-      }
+    for (int j = 0; j < kWords; ++j) w[j] = 0;
+    if (i + 8 <= 0 || i >= n) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i + j < 0 || i + j >= n) continue;
+      if constexpr (E == kElemF32) w[j] = static_cast<const uint32_t*>(p)[row + i + j];
+      else w[j >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[row + i + j]) << (16 * (j & 1));
     }
   }
   OGB_DEVICE void get(float (&f)[8]) const {
@@ -209,8 +254,19 @@ struct RowCode {
     return none ? make_uint2(0, 0) : bytes(u);
   }
 };
-// Codes from column i on; rows of q are a multiple of 16 bytes long, so that the last ones may pass the row's end.
+// Eight codes from column i on; rows of q are a multiple of 16 bytes long, so that the last ones may pass the row's end.
 OGB_DEVICE void store_codes(int8_t* q, size_t row, int i, uint2 codes) { *reinterpret_cast<uint2*>(q + row + i) = codes; }
+// The codes of a row whose pieces begin `shift` values in front of it: the eight of one piece from its `shift`-th on, then of the next.
+OGB_DEVICE uint2 shift_codes(uint2 a, uint2 b, int shift) {
+  const int bits = 8 * (shift & 3);
+  if (shift < 4) return make_uint2(__funnelshift_r(a.x, a.y, bits), __funnelshift_r(a.y, b.x, bits));
+  return make_uint2(__funnelshift_r(a.y, b.x, bits), __funnelshift_r(b.x, b.y, bits));
+}
+OGB_DEVICE void store_codes_strided(int8_t* q, size_t row, int i, int step, int n, uint2 codes) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (i + j * step < n) q[row + i + j * step] = static_cast<int8_t>((j < 4 ? codes.x >> (8 * j) : codes.y >> (8 * (j - 4))) & 255u);
+}
 OGB_DEVICE uint32_t peak_bits8(const float (&f)[8]) {
   uint32_t m = 0;
 #pragma unroll

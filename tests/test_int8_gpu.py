@@ -37,7 +37,8 @@ def _weight(g, n, k):
 
 
 @pytest.mark.parametrize("m,k,dtype,pad", [(1, 1, F32, 0), (3, 7, BF16, 0), (5, 8, F16, 3), (1, 3584, BF16, 0), (700, 896, BF16, 8), (33, 1001, F16, 0),
-                                           (1, 18944, BF16, 0), (2, 70000, F32, 1), (600, 4864, F32, 0), (400, 20001, BF16, 0)])
+                                           (1, 18944, BF16, 0), (2, 70000, F32, 1), (600, 4864, F32, 0), (400, 20001, BF16, 0), (3000, 897, BF16, 0), (500, 3583, F16, 0),
+                                           (700, 1001, F32, 0), (300, 16383, BF16, 0), (310, 32761, F16, 0), (309, 32767, BF16, 0), (2000, 50, F32, 1), (1, 8191, BF16, 0)])
 def test_rows_are_the_formula_bit_by_bit(m, k, dtype, pad):
     x = _rows(_gen(m + k), m, k, dtype, pad)
     r = int8.quantize_rows(x)
@@ -204,9 +205,10 @@ def _norm_want(x, y, kw, eps, xs, ys, sigmoid):
 
 
 @pytest.mark.parametrize("m,n,pad", [(1, 1, 0), (1, 3584, 0), (3, 33, 0), (600, 64, 8), (700, 896, 0), (5, 1001, 0), (400, 3584, 0), (310, 8192, 8), (2, 16384, 0),
-                                     (350, 16383, 0)])
+                                     (350, 16383, 0), (2000, 897, 0), (700, 3583, 0), (320, 8191, 0), (1500, 203, 0), (310, 10003, 0), (400, 130, 4), (900, 1024, 0)])
 @pytest.mark.parametrize("stream,dtype,post,gate,wtype", [(BF16, BF16, True, "channel", F32), (F32, BF16, True, "token", F32), (F32, F16, False, "none", F16),
-                                                          (F16, F32, True, "token", BF16)])
+                                                          (F16, F32, True, "token", BF16), (F32, F32, True, "token", F32), (BF16, F16, True, "channel", BF16),
+                                                          (BF16, F32, False, "none", F32)])
 def test_block_norm(m, n, pad, stream, dtype, post, gate, wtype):
     g = _gen(m * 31 + n)
     x, y, kw = _norm_case(g, m, n, stream, dtype, post, gate, wtype, pad)
