@@ -6,9 +6,11 @@
 // x is the residual stream, y what a block wrote, h what the next one reads: in a float type, or as 8-bit rows for a product.  All of it in
 // 32 bits from the loads to one rounding at each store; h is taken from x' before x' is rounded to the stream's type.
 //
-// Both are bound by the bytes they move.  A row stays in registers from its load to its last store, so nothing is read twice: a warp, or a
-// block of as many threads as leave each at most kNormVec pieces of eight values.  Few rows (a decode step) take a piece a thread, as
-// the time is then a chain of latencies -- load, three sums over the row, store -- and not bandwidth.
+// Both are bound by the bytes they move, and by the chain load - sums over the row - store where rows are few.  A row belongs to a block (short ones of
+// many to a warp) and stays in registers from its load to its last store, so nothing is read twice.  Rows up to two an SM take one piece of eight
+// values a thread, which makes the chain short; many rows take two or four, whose loads overlap.  The norm's next row comes through shared memory
+// while this one is summed and stored: 8192 rows of 3584 with a 32-bit stream, bf16 y, gate and h take 74 us, 5.6 TB/s of a copy's 6.45 (with a
+// row's loads behind the stores of the one before 82, with two whole rows in shared memory, and so fewer blocks, 106).
 #include <stdint.h>
 #include <string.h>
 
@@ -200,9 +202,7 @@ struct BlockNormParams {
   int rows, cols;
   int x_elem, y_elem, gate_elem, w_elem, h_elem;
   int gate_sigmoid;
-  int xo_wide, h_wide;                         // 32-byte stores (of 32-bit values)
   int shifted;                                 // rows do not all begin at multiples of eight values
-  int stages;                                  // rows in shared memory: this one and the next, or this one
   float eps, x_scale, y_scale;
 };
 
@@ -295,8 +295,9 @@ OGB_DEVICE float sigmoid_approx(float g) {
 }
 
 // Eight weights from column i on, wherever that is.
+template <bool SHIFT>
 OGB_DEVICE void load_weights(const void* p, int elem, int i, int n, float (&t)[8]) {
-  if ((i & 7) != 0) {                                                          // rows that are shifted against them
+  if (SHIFT && (i & 7) != 0) {                                                          // rows that are shifted against them
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[j] = i + j >= 0 && i + j < n ? load_elem(p, elem, i + j) : 0.f;
   } else if (elem == kElemF32) {
@@ -314,23 +315,25 @@ OGB_DEVICE void load_weights(const void* p, int elem, int i, int n, float (&t)[8
   }
 }
 // Eight results from column i on, one by one at the ends of a row.
-template <int E>
-OGB_DEVICE void store_piece(void* p, size_t row, int i, int n, bool wide, const float (&f)[8]) {
-  if (i >= 0 && i + 8 <= n) {
-    if (E == kElemF32 && wide) store32(static_cast<float*>(p) + row + i, f);
+template <int E, bool SHIFT>
+OGB_DEVICE void store_piece(void* p, size_t row, int i, int n, const float (&f)[8]) {
+  if ((!SHIFT || i >= 0) && i + 8 <= n) {
+    if (E == kElemF32) store32(static_cast<float*>(p) + row + i, f);
     else store8(p, E, true, row, i, n, f);
     return;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (i + j >= 0 && i + j < n) store_elem(p, E, row + i + j, f[j]);
+    if ((!SHIFT || i + j >= 0) && i + j < n) store_elem(p, E, row + i + j, f[j]);
 }
 
 // The same for matrices that begin at multiples of eight values and share a row stride modulo eight (contiguous ones do): every row is taken in pieces of
 // eight values that lie at such multiples in all of them.  XE: type of the stream, YE: of the block's output, a gate a token and h.  Weights meet the values
 // before the sum over the row is known, so that what follows a sum is one product; the largest |h| is the largest |x' pre| times the root, so it joins the
-// second sum's exchange.  The row comes through shared memory, and the next one with it where there is room.
-template <int XE, int YE, int V, int T>
+// second sum's exchange.  A warp's pieces come through shared memory by copies of its own: those of the next row's y and gate start once this row's have been
+// read, those of its stream once x' is formed, so that loads pass under the sums and stores.  SHIFT: rows do not all begin at multiples of
+// eight values (8192 x 3583: 113 us; where they do, 3584: 74).
+template <int XE, int YE, int V, int T, bool SHIFT>
 __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_norm_usual_kernel(const BlockNormParams p) {
   __shared__ __align__(16) float part_y[2][kMostThreads / 32], part_x[2][kMostThreads / 32];
   __shared__ __align__(16) uint32_t part_q[2][kMostThreads / 32];
@@ -359,26 +362,29 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
 #pragma unroll
       for (int h = 0; h < kW; ++h) {
         const int w = lane + 32 * h, piece = (tid - lane) * 8 + v * step - shift + 8 * (w / kW);
-        if (piece >= 0 && piece + 8 <= n)
+        if ((!SHIFT || piece >= 0) && piece + 8 <= n)
           copy(to + (v * kW * all + (kW == 2 ? w ^ (w >> 3 & 1) : w)) * 16, s + (at + piece) * kBytes + (w % kW) * 16);
       }
   };
   using XBytes = std::integral_constant<int, kXBytes>;
   using YBytes = std::integral_constant<int, kYBytes>;
-  auto fetch = [&](int row, int stage) {
-    const int shift = row_shift(row, p.ldx);
-    const uint32_t to = base + stage * words * all * 16;
-    // (a warp's 64 words lie next to one another, a block's two sets of 32 a thread apart: every warp's begin at twice its first thread's)
-    fetch_matrix(XBytes(), to + (kX == 2 ? (threadIdx.x - lane) * 16 : 0), x, static_cast<size_t>(row) * p.ldx, shift);
-    if (has_y) fetch_matrix(YBytes(), to + V * kX * all * 16 + (kY == 2 ? (threadIdx.x - lane) * 16 : 0), y, static_cast<size_t>(row) * p.ldy, shift);
-    if (gate_row) fetch_matrix(YBytes(), to + V * (kX + kY) * all * 16 + (kY == 2 ? (threadIdx.x - lane) * 16 : 0), g, static_cast<size_t>(row) * p.ldg, shift);
+  // (a warp's 64 words lie next to one another, a block's two sets of 32 a thread apart: every warp's begin at twice its first thread's)
+  auto fetch_x = [&](int row) {
+    fetch_matrix(XBytes(), base + (kX == 2 ? (threadIdx.x - lane) * 16 : 0), x, static_cast<size_t>(row) * p.ldx, SHIFT ? row_shift(row, p.ldx) : 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto fetch_y = [&](int row) {
+    const int shift = SHIFT ? row_shift(row, p.ldx) : 0;
+    const uint32_t to = base + V * kX * all * 16 + (kY == 2 ? (threadIdx.x - lane) * 16 : 0);
+    if (has_y) fetch_matrix(YBytes(), to, y, static_cast<size_t>(row) * p.ldy, shift);
+    if (gate_row) fetch_matrix(YBytes(), to + V * kY * all * 16, g, static_cast<size_t>(row) * p.ldg, shift);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // piece v of a matrix whose words begin at `from` of this warp's
   auto get = [&](auto elem, const uint4* from, int v, const char* s, size_t at, int i, float (&t)[8]) {
     constexpr int E = decltype(elem)::value;
     Raw8<E> r;
-    if (i < 0 || i + 8 > n) {
+    if ((SHIFT && i < 0) || i + 8 > n) {
       r.edge(s, at, i, n);
     } else if constexpr (E == kElemF32) {
       const uint4* two = from + (threadIdx.x - lane) + v * 2 * all + 2 * lane;
@@ -394,16 +400,14 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
   using XElem = std::integral_constant<int, XE>;
   using YElem = std::integral_constant<int, YE>;
   int row = blockIdx.x * warps + (WARP ? threadIdx.x >> 5 : 0);
-  if (p.stages == 2 && row < p.rows) fetch(row, 0);
+  if (row < p.rows) {
+    fetch_y(row);
+    fetch_x(row);
+  }
   for (int turn = 0; row < p.rows; row += rows_step, turn ^= 1) {
-    __syncwarp();                                                             // what the copies overwrite has been read by the whole warp
-    if (p.stages == 1) fetch(row, 0);
-    else if (row + rows_step < p.rows) fetch(row + rows_step, turn ^ 1);
-    if (p.stages == 2 && row + rows_step < p.rows) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncwarp();
-    const uint4* from = mine + (p.stages == 2 ? turn * words * all : 0);
-    const int i0 = tid * 8 - row_shift(row, p.ldx);
+    const int i0 = tid * 8 - (SHIFT ? row_shift(row, p.ldx) : 0);
     float a[V][8], ry = p.y_scale;
     if (has_y) {
       float sum = 0.f;
@@ -412,9 +416,9 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
         const int i = i0 + v * step;
         if (i < n) {
           float t[8];
-          get(YElem(), from + V * kX * all, v, y, static_cast<size_t>(row) * p.ldy, i, a[v]);
+          get(YElem(), mine + V * kX * all, v, y, static_cast<size_t>(row) * p.ldy, i, a[v]);
           if (p.post != nullptr) {
-            load_weights(p.post, p.w_elem, i, n, t);
+            load_weights<SHIFT>(p.post, p.w_elem, i, n, t);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               sum = fmaf(a[v][j], a[v][j], sum);
@@ -422,8 +426,8 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
             }
           }
           if (g != nullptr) {
-            if (gate_row) get(YElem(), from + V * (kX + kY) * all, v, g, static_cast<size_t>(row) * p.ldg, i, t);
-            else load_weights(g, p.gate_elem, i, n, t);
+            if (gate_row) get(YElem(), mine + V * (kX + kY) * all, v, g, static_cast<size_t>(row) * p.ldg, i, t);
+            else load_weights<SHIFT>(g, p.gate_elem, i, n, t);
             if (p.gate_sigmoid != 0) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) t[j] = sigmoid_approx(t[j]);
@@ -433,8 +437,15 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
           }
         }
       }
+      __syncwarp();                                                           // the whole warp has read what the copies overwrite
+      if (row + rows_step < p.rows) fetch_y(row + rows_step);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
       if (p.post != nullptr) ry *= rsqrtf(row_sum<WARP>(sum, part_y[turn]) * over + p.eps);
+    } else {
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
     float sum = 0.f;
     uint32_t peak = 0;
 #pragma unroll
@@ -442,16 +453,16 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
       const int i = i0 + v * step;
       if (i < n) {
         float t[8];
-        get(XElem(), from, v, x, static_cast<size_t>(row) * p.ldx, i, t);      // zeros in front of a row and past its end, and so is x'
+        get(XElem(), mine, v, x, static_cast<size_t>(row) * p.ldx, i, t);      // zeros in front of a row and past its end, and so is x'
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           t[j] *= p.x_scale;
           if (has_y) t[j] = fmaf(ry, a[v][j], t[j]);
           a[v][j] = t[j];
         }
-        if (p.x_out != nullptr) store_piece<XE>(p.x_out, static_cast<size_t>(row) * p.ldxo, i, n, p.xo_wide != 0, a[v]);
+        if (p.x_out != nullptr) store_piece<XE, SHIFT>(p.x_out, static_cast<size_t>(row) * p.ldxo, i, n, a[v]);
         if (p.pre != nullptr) {
-          load_weights(p.pre, p.w_elem, i, n, t);
+          load_weights<SHIFT>(p.pre, p.w_elem, i, n, t);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             sum = fmaf(a[v][j], a[v][j], sum);
@@ -461,6 +472,8 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
         if (p.q != nullptr) peak = max(peak, peak_bits8(a[v]));
       }
     }
+    __syncwarp();
+    if (row + rows_step < p.rows) fetch_x(row + rows_step);
     if (p.h == nullptr && p.q == nullptr) continue;
     float rx = 1.f;
     if (p.q != nullptr) {
@@ -477,7 +490,7 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
         if (i < n) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) a[v][j] *= rx;
-          store_piece<YE>(p.h, static_cast<size_t>(row) * p.ldh, i, n, p.h_wide != 0, a[v]);
+          store_piece<YE, SHIFT>(p.h, static_cast<size_t>(row) * p.ldh, i, n, a[v]);
         }
       }
       continue;
@@ -495,12 +508,12 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[v][j] *= rx;
         codes[v] = code.codes(a[v]);
-        if (p.shifted == 0) store_codes(p.q, static_cast<size_t>(row) * p.ldq, i0 + v * step, codes[v]);
+        if (!SHIFT) store_codes(p.q, static_cast<size_t>(row) * p.ldq, i0 + v * step, codes[v]);
       }
     }
-    if (p.shifted != 0) {
+    if (SHIFT) {
       // a word of q is made of two pieces: the next one is the next thread's
-      uint2* exchange = reinterpret_cast<uint2*>(slots + p.stages * words * all) + (WARP ? (threadIdx.x >> 5) * (32 * V + 1) : 0);
+      uint2* exchange = reinterpret_cast<uint2*>(slots + words * all) + (WARP ? (threadIdx.x >> 5) * (32 * V + 1) : 0);
       if (WARP) __syncwarp();
       else __syncthreads();                                                   // of the row before
 #pragma unroll
@@ -524,20 +537,17 @@ static int launch_norm_kernel(OncePerDevice& allowed, Kernel kernel, BlockNormPa
   auto words = [](const void* m, int elem) { return m == nullptr ? 0 : elem == kElemF32 ? 2 : 1; };
   const int block = T == 32 ? 128 : threads;
   const int stage = 16 * block * V * (words(p.x, p.x_elem) + words(p.y, p.y_elem) + (p.ldg != 0 ? words(p.gate, p.gate_elem) : 0));
-  // The next row's copies pass under this row's sums where shared memory holds both rows of as many blocks as registers do; else more blocks do
-  // better (8192 rows of 3584, stream in 32 bits with a gate a token: 106 us with three blocks of two rows, 92 with four of one).
   const int most = std::max(1, 65536 / ((V < kVec ? 64 : 80) * block));
-  p.stages = (2 * stage + 1024) * most <= kNormSmem ? 2 : 1;
   const int exchange = p.q != nullptr && p.shifted != 0 ? (8 * (T == 32 ? 4 * (32 * V + 1) : V * block + 1) + 15) / 16 * 16 : 0;
-  const int smem = p.stages * stage + exchange;
+  const int smem = stage + exchange;
   const int per_sm = std::max(1, std::min(kNormSmem / (smem + 1024), most));
   const int grid = std::min(T == 32 ? (p.rows + 3) / 4 : p.rows, ogb_num_sms() * per_sm);
   return static_cast<int>(launch_overlapped(kernel, dim3(grid), dim3(block), smem, stream, p));
 }
-template <int V, int T>
+template <int V, int T, bool SHIFT>
 static int launch_usual(const BlockNormParams& p, int threads, cudaStream_t stream) {
   static OncePerDevice allowed[6];
-#define OGB_NORM(AT, XE, YE) return launch_norm_kernel<V, T>(allowed[AT], block_norm_usual_kernel<XE, YE, V, T>, p, threads, stream)
+#define OGB_NORM(AT, XE, YE) return launch_norm_kernel<V, T>(allowed[AT], block_norm_usual_kernel<XE, YE, V, T, SHIFT>, p, threads, stream)
   if (p.x_elem == kElemF32) {
     if (p.y_elem == kElemF32) OGB_NORM(0, kElemF32, kElemF32);
     if (p.y_elem == kElemBf16) OGB_NORM(1, kElemF32, kElemBf16);
@@ -572,9 +582,13 @@ static int launch_norm(BlockNormParams p, cudaStream_t stream) {
   p.y_elem = side;
   p.shifted = p.ldx % 8 != 0 ? 1 : 0;
   const int cols = p.cols + (p.shifted != 0 ? 7 : 0), t = row_threads(p.rows, cols, 2), pieces = (cols + 7) / 8;
-  if (t == 32) return launch_usual<2, 32>(p, t, stream);
-  if (pieces <= t) return launch_usual<1, kMostThreads>(p, t, stream);
-  return pieces <= 2 * t ? launch_usual<2, kMostThreads>(p, t, stream) : launch_usual<kVec, kMostThreads>(p, t, stream);
+  auto launch = [&](auto shifted) {
+    constexpr bool S = decltype(shifted)::value;
+    if (t == 32) return launch_usual<2, 32, S>(p, t, stream);
+    if (pieces <= t) return launch_usual<1, kMostThreads, S>(p, t, stream);
+    return pieces <= 2 * t ? launch_usual<2, kMostThreads, S>(p, t, stream) : launch_usual<kVec, kMostThreads, S>(p, t, stream);
+  };
+  return p.shifted != 0 ? launch(std::true_type()) : launch(std::false_type());
 }
 
 }  // namespace ogb
@@ -598,7 +612,7 @@ extern "C" int ogb_block_norm(const void* x, const void* y, const void* gate, co
   if (rows == 0) return 0;
   if (q != nullptr && (ldq < cols || (ldq & 15) != 0 || (reinterpret_cast<uintptr_t>(q) & 15) != 0 || factor == nullptr)) return -3;
   const BlockNormParams p{x, y, gate, post, pre, x_out, h, static_cast<int8_t*>(q), factor, ldx, ldy, ldg, ldxo, ldh, ldq, rows, cols, x_elem, y_elem, gate_elem,
-                          w_elem, h_elem, gate_sigmoid, 1, 1, 0, 2, eps, x_scale, y_scale};
+                          w_elem, h_elem, gate_sigmoid, 0, eps, x_scale, y_scale};
   return launch_norm(p, static_cast<cudaStream_t>(stream_));
 }
 

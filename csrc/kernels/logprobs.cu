@@ -204,7 +204,7 @@ template <typename T>
 OGB_DEVICE void lp_load(const T* x, int i0, int vocab, uint32_t (&w)[8]) {
   using Type = LpType<T>;
   if (i0 >= 0 && i0 + Type::kPer <= vocab) {
-    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                  : "l"(x + i0));
     return;

@@ -53,6 +53,12 @@ _SIGNATURES = {
     "ogb_sample_bf16": ([P, P, P, P, P, P, P, P, I, I, I, P], I),
     "ogb_token_logprobs_args": ([ctypes.c_char_p], I),
     "ogb_token_logprobs": ([P] * 7 + [I, I, L, I, I, P, P], I),
+    "ogb_quantize_rows": ([P] * 3 + [I] * 2 + [L] * 2 + [I, P], I),
+    "ogb_gemm_int8_workspace": ([I] * 5, L),
+    "ogb_gemm_int8_args": ([ctypes.c_char_p], I),
+    "ogb_gemm_int8": ([P, I, L, P, P, L, P, L, P, P, P, L, P, L] + [I] * 5 + [P, L, P, P], I),
+    "ogb_block_norm_args": ([ctypes.c_char_p], I),
+    "ogb_block_norm": ([P] * 9 + [L] * 6 + [I] * 8 + [F] * 3 + [P], I),
     "ogb_spec_verify_greedy": ([P, P, P, P, I, I, I, I, P], I),
     "ogb_kv_page_copy": ([P, P, P, I, L, P], I),
     "ogb_kv_gather_pages": ([P, P, P, I, L, P], I),

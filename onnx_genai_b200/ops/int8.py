@@ -8,7 +8,6 @@ the statements of :mod:`onnx_genai_b200.ops.reference`.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 import struct
 from typing import NamedTuple
@@ -16,14 +15,6 @@ from typing import NamedTuple
 import torch
 
 from . import _native, _raw_stream, _timed, current_index, launch_counts, reference, status_ptr
-
-P, I, L, F = _native.P, _native.I, _native.L, _native.F
-_native.register("ogb_gemm_int8_args", [ctypes.c_char_p])
-_native.register("ogb_block_norm_args", [ctypes.c_char_p])
-_native.register("ogb_quantize_rows", [P] * 3 + [I] * 2 + [L] * 2 + [I, P])
-_native.register("ogb_gemm_int8_workspace", [I] * 5, L)
-_native.register("ogb_gemm_int8", [P, I, L, P, P, L, P, L, P, P, P, L, P, L] + [I] * 5 + [P, L, P, P])
-_native.register("ogb_block_norm", [P] * 9 + [L] * 6 + [I] * 8 + [F] * 3 + [P])
 
 ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_K = 131072          # sums of 128 * 127 * K stay below 2^31
@@ -109,9 +100,9 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     out [M, N / 2]).
 
     ``a`` [M, K]: float rows, which the call turns into 8 bits (:func:`quantize_rows`), or :class:`Int8Rows`.  ``w`` [N, K] int8, rows at
-    multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.  ``residual`` has the type of the result; ``out`` may be the same tensor.  The result's
-    type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else bf16.  Sums over K are exact; one rounding follows the
-    factors, the bias and the residual."""
+    multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.  ``residual`` has the type of the result; ``out`` may be the same tensor, and
+    shares no memory with ``a`` and ``w``.  The result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else
+    bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
     rows = isinstance(a, Int8Rows)
     x = a.q if rows else a
     gated = epilogue == "swiglu"
@@ -144,10 +135,15 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     out_kind = ELEM.get(out_dtype)
     if out_kind is None:
         _refuse(f"results of {out_dtype}")
-    if out is not None:
-        _result(out, m, n_out, out_dtype, dev)
     if residual is not None:
         _result(residual, m, n_out, out_dtype, dev)
+    if out is not None:
+        _result(out, m, n_out, out_dtype, dev)
+        place = _place(out)
+        if _meet(*place, *_place(x)) or _meet(*place, *_place(w)):
+            _refuse("out shares memory with a or w")
+        if residual is not None and _meet(*place, *_place(residual)) and (out.data_ptr() != residual.data_ptr() or out.stride() != residual.stride()):
+            _refuse("out is the residual itself or shares no memory with it")
     if not x.is_cuda:
         y = reference.gemm_int8(a, w, w_scale, bias, residual, gated, out_dtype)
         return y if out is None else out.copy_(y)
@@ -194,6 +190,24 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     return out
 
 
+def _meet(a, rows_a, pitch_a, width_a, b, rows_b, pitch_b, width_b) -> bool:
+    """Whether two matrices share memory (addresses, and pitches and widths in bytes); columns side by side in rows of one pitch do not."""
+    if a > b:
+        a, rows_a, pitch_a, width_a, b, rows_b, pitch_b, width_b = b, rows_b, pitch_b, width_b, a, rows_a, pitch_a, width_a
+    if rows_a == 0 or rows_b == 0 or b >= a + (rows_a - 1) * pitch_a + width_a:
+        return False
+    if pitch_a == pitch_b > 0:
+        beside = (b - a) % pitch_a
+        return beside < width_a or beside + width_b > pitch_a
+    return True
+
+
+def _place(t):
+    """A matrix for :func:`_meet`."""
+    size, (rows, cols), (ld, step) = t.element_size(), t.shape, t.stride()
+    return t.data_ptr(), rows if cols else 0, ld * size, ((cols - 1) * step + 1) * size
+
+
 def _result(t, m, n, dtype, dev):
     if t.shape != (m, n) or t.dtype is not dtype or t.device != dev or (n > 1 and t.stride(1) != 1):
         _refuse(f"out and residual: [{m}, {n}] {dtype} with neighbouring columns on the device of a")
@@ -215,10 +229,11 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     """The step between two blocks of a decoder: ``x' = x_scale * x + y_scale * g * post(y)``, then ``h = pre(x')``, which is returned.
 
     ``x`` [rows, hidden]: the residual stream (fp32, bf16, fp16), replaced by x' unless ``x_out`` (same type) takes it.  ``y``: what the block
-    wrote (None: nothing is added; the stream stays as it is unless ``x_out`` or ``x_scale`` says otherwise).  ``post`` and ``pre``: weights [hidden] of RMS norms in one
-    type (None: no norm).  ``gate``: [hidden] or [rows, hidden], taken as it is or through a sigmoid.  ``h`` comes in ``out_dtype`` (that of ``out``, else of ``x``), or as
-    :class:`Int8Rows` with ``int8=True``.  All of it is computed in 32 bits and rounded where it is stored; h is taken from x' before that is
-    rounded.  ``hidden`` is at most 16384 on CUDA; the tensors' columns are neighbours."""
+    wrote (None: nothing is added; the stream stays as it is unless ``x_out`` or ``x_scale`` says otherwise).  ``post`` and ``pre``: weights
+    [hidden] of RMS norms in one type (None: no norm).  ``gate``: [hidden] or [rows, hidden], taken as it is or through a sigmoid.  ``h`` comes
+    in ``out_dtype`` (that of ``out``, else of ``x``), or as :class:`Int8Rows` with ``int8=True``.  ``x_out`` and ``out`` may each be a matrix
+    that is read; otherwise they share memory with nothing.  All of it is computed in 32 bits and rounded where it is stored; h is taken from x'
+    before that is rounded.  ``hidden`` is at most 16384 on CUDA; the tensors' columns are neighbours."""
     shape, dev, dtype = x.shape, x.device, x.dtype
     kind = ELEM.get(dtype)
     if kind is None or len(shape) != 2:
@@ -270,6 +285,18 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
             ldo = _matrix(out, shape, dev)
             if ldo < n and rows > 1:
                 _refuse("rows of out overlap")
+    # a matrix that is written may stand in the place of one that is read, row for row; any other meeting would change what is still to be read
+    x_ptr = x.data_ptr()
+    wide, y_wide, gate_wide = (4 if k == 0 else 2 for k in (kind, y_kind, gate_kind))
+    reads = (x_ptr, ldx, kind, wide), (y_ptr, ldy, y_kind, y_wide), (gate_ptr if ldg else 0, ldg, gate_kind, gate_wide)
+    if new_ptr:
+        _separate(new_ptr, ldn, kind, wide, reads, rows, n)
+    if out is not None:
+        out_kind, out_ptr = ELEM[out_dtype], out.data_ptr()
+        out_wide = 4 if out_kind == 0 else 2
+        _separate(out_ptr, ldo, out_kind, out_wide, reads, rows, n)
+        if new_ptr and _meet(new_ptr, rows, ldn * wide, n * wide, out_ptr, rows, ldo * out_wide, n * out_wide):
+            _refuse("the new stream and out share memory")
     if not x.is_cuda:
         new, h = reference.block_norm(x, y, post, gate, pre, eps, x_scale, y_scale, gate_sigmoid)
         if int8:
@@ -294,15 +321,23 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     else:
         if out is None:
             out, ldo = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=dev), n
+            out_kind, out_ptr = ELEM[out_dtype], out.data_ptr()
         q_ptr = ldq = scale_ptr = 0
-        out_ptr, out_kind = out.data_ptr(), ELEM[out_dtype]
-    rc = _native.load().ogb_block_norm_args(_pack_norm(x.data_ptr(), y_ptr, gate_ptr, post_ptr, pre_ptr, new_ptr, out_ptr, q_ptr, scale_ptr, ldx, ldy, ldg, ldn, ldo,
+    rc = _native.load().ogb_block_norm_args(_pack_norm(x_ptr, y_ptr, gate_ptr, post_ptr, pre_ptr, new_ptr, out_ptr, q_ptr, scale_ptr, ldx, ldy, ldg, ldn, ldo,
                                                        ldq, rows, n, kind, y_kind, gate_kind, w_kind, out_kind, gate_sigmoid, eps, x_scale, y_scale,
                                                        _raw_stream(index)))
     if rc:
         _native.check(rc, "ogb_block_norm")
     launch_counts["block_norm"] += 1
     return Int8Rows(q, scale) if int8 else out
+
+
+def _separate(ptr, ld, kind, wide, reads, rows, n):
+    end = ptr + ((rows - 1) * ld + n) * wide
+    for other, ldr, other_kind, other_wide in reads:
+        if other < end and ptr < other + ((rows - 1) * ldr + n) * other_wide and _meet(ptr, rows, ld * wide, n * wide, other, rows, ldr * other_wide, n * other_wide):
+            if ptr != other or kind != other_kind or (ld != ldr and rows > 1):
+                _refuse("x_out (or x) and out: matrices that share memory with none, or the very ones that are read")
 
 
 def _matrix(t, shape, dev):

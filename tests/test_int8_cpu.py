@@ -134,3 +134,24 @@ def test_what_log_probabilities_refuse():
                  dict(logits=x, tokens=torch.zeros(2).int(), top=-1), dict(logits=x[:, :0], tokens=torch.zeros(2).int())):
         with pytest.raises(ValueError):
             ops.token_logprobs(**args)
+
+
+def test_results_that_share_memory_are_refused():
+    buf = torch.zeros(4, 64)
+    x, w = buf[:2, :32], int8.quantize_weight(_rand(32, 32))
+    for out in (x, buf[1:3, :32], buf[:2, 16:48]):
+        with pytest.raises(ValueError):
+            int8.gemm_int8(x, w.q, w.scale, out=out)
+    with pytest.raises(ValueError):
+        int8.gemm_int8(_rand(2, 32), w.q, w.scale, residual=buf[:2, :32], out=buf[:2, 8:40])
+    assert int8.gemm_int8(_rand(2, 32), w.q, w.scale, residual=x, out=x) is x
+    beside = buf[:2, 32:]                                            # columns of one buffer, side by side
+    assert torch.equal(int8.gemm_int8(x, w.q, w.scale, out=beside), int8.gemm_int8(x, w.q, w.scale))
+    assert int8.block_norm(x, _rand(2, 32), out=beside) is beside
+    y = _rand(2, 32)
+    for kw in (dict(out=buf[1:3, :32]), dict(x_out=buf[:2, 8:40]), dict(x_out=y, out=y), dict(x_out=torch.empty(3, 32)[:2], out=x, y=y[:, :0])):
+        with pytest.raises(ValueError):
+            int8.block_norm(x, **{"y": y, **kw})
+    keep = x.clone()
+    want = int8.block_norm(keep, y.clone(), pre=torch.ones(32))
+    assert torch.equal(int8.block_norm(x, y, pre=torch.ones(32), out=y), want) and torch.equal(x, keep)      # h in the place of y

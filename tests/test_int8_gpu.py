@@ -325,3 +325,17 @@ def test_products_inside_a_step_whose_kernels_start_early():
         got = step(x)
     assert torch.equal(got, want)
     ops.check_status()
+
+
+@pytest.mark.parametrize("m,n", [(700, 897), (300, 3584), (5, 64), (900, 50)])
+def test_norms_in_the_place_of_what_they_read(m, n):
+    g = _gen(m)
+    x, y, kw = _norm_case(g, m, n, BF16, BF16, True, "token", F32)
+    new = torch.empty_like(x)
+    h = int8.block_norm(x, y, x_out=new, gate_sigmoid=True, **kw)
+    a, b = x.clone(), y.clone()
+    assert int8.block_norm(a, b, out=b, gate_sigmoid=True, **kw) is b
+    assert torch.equal(a, new) and torch.equal(b, h)
+    a, b = x.clone(), y.clone()
+    rows = int8.block_norm(a, b, x_out=b, gate_sigmoid=True, int8=True, **kw)
+    assert torch.equal(a, x) and torch.equal(b, new) and torch.equal(rows.q, int8.block_norm(x, y, x_out=new, gate_sigmoid=True, int8=True, **kw).q)
