@@ -279,7 +279,8 @@ class Engine:
         plan = procs.device_sampling_plan(chain, eff, sampler is not None)
         # Greedy requests whose only wish beyond the device's own path are log probabilities get them there (ops.token_logprobs); a row of
         # logits does not cross to the host.
-        on_device = (opt.logprobs and self.llm.device.type == "cuda" and self.llm.tp == 1 and self.llm.pp == 1 and not opt.speculative
+        on_device = (0 < opt.logprobs <= self.llm.cfg.model.vocab and not opt.speculative
+                     and self.llm.device.type == "cuda" and self.llm.tp == 1 and self.llm.pp == 1
                      and procs.device_sampling_plan(chain, GenerateOptions(**{**eff.__dict__, "logprobs": 0}), sampler is not None) == "greedy")
         if on_device:
             plan = "greedy"

@@ -335,6 +335,7 @@ class LLMEngine:
         if self.has_work or self.stats or self.forced:
             raise RuntimeError("score() drives the engine by itself: finish the requests in flight first")
         rows = self.logit_row_limit
+        empty = ops.token_logprobs(torch.zeros(0, self.cfg.model.vocab), torch.zeros(0, dtype=torch.int32), top, entropy)      # refuses what a step would
         results = []
         for tokens in prompts:
             tokens = [int(t) for t in tokens]
@@ -358,7 +359,6 @@ class LLMEngine:
                 if sid is not None:
                     self.scoring.pop(sid, None)
                     self.close_forced(sid)
-            empty = ops.token_logprobs(torch.zeros(0, self.cfg.model.vocab), torch.zeros(0, dtype=torch.int32), top, entropy)
             results.append(ops.TokenLogprobs(*(None if e is None else torch.cat([e] + [p[i].cpu() for p in parts]) for i, e in enumerate(empty))))
         return results
 

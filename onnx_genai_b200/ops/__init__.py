@@ -581,6 +581,8 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
     rows, vocab = shape
     if not 0 <= top <= (MAX_TOP_LOGPROBS if vocab > MAX_TOP_LOGPROBS else vocab):
         raise ValueError(f"top = {top}: between 0 and {min(MAX_TOP_LOGPROBS, vocab)}")
+    if rows > 1 << 30:
+        raise ValueError(f"{rows} rows: at most {1 << 30}")
     if vocab > MAX_VOCAB_WITH_TOP and (top or vocab > MAX_VOCAB):
         raise ValueError(f"a vocabulary of {vocab}: at most {MAX_VOCAB_WITH_TOP if top else MAX_VOCAB}")
     dev = logits.device

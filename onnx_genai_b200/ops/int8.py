@@ -18,6 +18,7 @@ from . import _native, _raw_stream, _timed, current_index, launch_counts, refere
 
 ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_K = 131072          # sums of 128 * 127 * K stay below 2^31
+MAX_ROWS = 1 << 30       # of rows and of channels
 MAX_HIDDEN = 16384      # a row of block_norm stays in registers
 _EPI = ("none", "residual", "swiglu")
 # arguments of the two calls with many, as 64-bit words (ctypes takes 2 us to convert them one by one)
@@ -54,8 +55,8 @@ def quantize_rows(x) -> Int8Rows:
     if x.dim() != 2 or x.dtype not in ELEM:
         _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(x.shape)} {x.dtype}")
     rows, k = x.shape
-    if k == 0:
-        _refuse("rows without values have no scale")
+    if not 0 < k < MAX_ROWS or rows > MAX_ROWS:
+        _refuse(f"{rows} rows of {k} values: at most {MAX_ROWS}, and at least one value")
     if k > 1 and x.stride(1) != 1:
         x = x.contiguous()
     dev = x.device
@@ -118,6 +119,8 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
         _refuse(f"rows of {dtype}")
     if not 0 < k <= MAX_K:
         _refuse(f"k = {k}: between 1 and {MAX_K}")
+    if m > MAX_ROWS or n > MAX_ROWS:
+        _refuse(f"{m} rows and {n} channels: at most {MAX_ROWS}")
     if w.dtype is not torch.int8 or w.device != dev:
         _refuse("w must be int8 on the device of a")
     if w_scale is None or not _channels(w_scale, n, dev) or not (bias is None or _channels(bias, n, dev)):
@@ -239,8 +242,8 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
     if kind is None or len(shape) != 2:
         _refuse(f"x must be a matrix of fp32, bf16 or fp16, not {tuple(shape)} {dtype}")
     rows, n = shape
-    if n == 0:
-        _refuse("rows without values")
+    if n == 0 or rows > MAX_ROWS:
+        _refuse(f"{rows} rows of {n} values: at most {MAX_ROWS}, and at least one value")
     ldx = _matrix(x, shape, dev)
     ldy = ldg = ldo = 0
     y_kind = gate_kind = w_kind = 0

@@ -155,3 +155,13 @@ def test_results_that_share_memory_are_refused():
     keep = x.clone()
     want = int8.block_norm(keep, y.clone(), pre=torch.ones(32))
     assert torch.equal(int8.block_norm(x, y, pre=torch.ones(32), out=y), want) and torch.equal(x, keep)      # h in the place of y
+
+
+def test_more_rows_than_the_kernels_count_are_refused():
+    many = torch.zeros(1, 16).expand(2**31, 16)
+    w = int8.quantize_weight(_rand(16, 16))
+    for call in (lambda: int8.quantize_rows(many), lambda: int8.gemm_int8(many, w.q, w.scale), lambda: int8.block_norm(many, x_scale=1.0),
+                 lambda: int8.gemm_int8(_rand(1, 16), torch.zeros(1, 16, dtype=torch.int8).expand(2**31, 16), torch.zeros(1).expand(2**31)),
+                 lambda: ops.token_logprobs(many, torch.zeros(1, dtype=torch.int32).expand(2**31))):
+        with pytest.raises(ValueError):
+            call()

@@ -339,3 +339,12 @@ def test_norms_in_the_place_of_what_they_read(m, n):
     a, b = x.clone(), y.clone()
     rows = int8.block_norm(a, b, x_out=b, gate_sigmoid=True, int8=True, **kw)
     assert torch.equal(a, x) and torch.equal(b, new) and torch.equal(rows.q, int8.block_norm(x, y, x_out=new, gate_sigmoid=True, int8=True, **kw).q)
+
+
+@pytest.mark.parametrize("m,n,k,gated,cut", [(20, 19072, 11000, False, True), (100, 20000, 15000, False, True), (40, 38400, 13000, True, True),
+                                             (3000, 5000, 14000, False, False), (8192, 3584, 18944, False, True)])
+def test_long_k_and_tiles_that_are_cut_into_ranges(m, n, k, gated, cut):
+    # cut where a few tiles more than fill the SMs: workspace beyond that for the rows
+    assert (int8._workspace(m, n, k, gated, False) > 0) is cut
+    _check_product(_gen(m + n), m, n, k, BF16, True, not gated, gated)
+    _check_product(_gen(m + k), m, n, k, F16, True, False, gated, as_rows=True)

@@ -75,6 +75,9 @@ def test_what_score_refuses():
             eng.score(bad)
     with pytest.raises(ValueError):
         eng.score([[1] * 300])
+    for top in (-1, 33):
+        with pytest.raises(ValueError):
+            eng.score([[1, 2, 3]], top=top)
     assert not eng.forced and not eng.scoring
     eng.add_request([1, 2, 3], 2)
     with pytest.raises(RuntimeError):
