@@ -8,17 +8,24 @@
 // kind::f16 for the same bytes of operands.
 //
 // W is the M side of tcgen05.mma -- 128 channels a tile, TW = 2: 128 gate and their 128 up channels, two accumulators -- and the rows are its N
-// side, padded to a multiple of 16 only, up to 256 (128 when gated).  So one kernel serves one row, whose stage of the ring is W almost
-// alone, and thousands, 128 x 256 to a tile.  Warp 0 issues the TMA loads, warp 1 the products, warps 2 - 5 the epilogue: sums leave
-// TMEM for shared memory 32 rows at a time and come back a row per warp, so that 128 channels of a row are stored together.
+// side, padded to a multiple of 16 only, up to 256 (128 when gated).  So one kernel serves three rows, whose stage of the ring is W almost
+// alone, and thousands, 128 x 256 to a tile (PAIR: 256 x 256 to two CTAs).  Warp 0 issues the TMA loads, warp 1 the products, warps 2 - 9 are two groups of
+// the epilogue: sums leave TMEM for shared memory 32 rows at a time and come back a row per warp, so that 128 channels of a row are stored
+// together.
 //
-// Division of the work:
+// Division of the work (i8_plan):
 //   * no more tiles than SMs: a cluster of up to 8 CTAs shares a tile, each takes a part of K; the parts are summed over distributed shared
 //     memory;
-//   * else: whole tiles, dealt to one CTA per SM in rounds, the epilogue of a tile under the products of the next (two accumulators).  The
-//     tiles left for the last round, which would leave most SMs idle, are cut along K into one range per SM; CTAs that share a tile leave
-//     their sums in a workspace, and whichever comes last adds them up.  Ranges come first, so that those sums pass under whole tiles.
+//   * else: whole tiles, dealt to one CTA (or pair) per SM in rounds, the epilogue of a tile under the products of the next (two accumulators).
+//     Where K is long the tiles left for the last round, which would leave most SMs idle, are cut along K into one range per SM; CTAs that
+//     share a tile leave their sums in a workspace, and whichever comes last adds them up.  Ranges come first, so that those sums pass under
+//     whole tiles;
+//   * one or two rows of a weight of moderate size: no tensor cores (gemv_int8_kernel).
+//
+// Measured with weights from HBM, 8-bit rows made by the call: 64 rows against 3584 x 18944 with a residual 22 us; 77, gated 37888 x 3584 31;
+// 8192, 3584 x 18944 rows 93 and product 347, 3.2 POP/s; one row of 4608 x 3584 7.4.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm_common.cuh"
@@ -48,7 +55,8 @@ struct Int8Params {
   const void* residual;                      // or null
   long long ldc, ldr;
   int vec;                                   // results and residuals in pieces of four
-  int M, N, mn;                              // mn: rows of a tile, a multiple of 16
+  int pair;                                  // 1: two CTAs on 256 channels
+  int M, N, mn;                              // mn: rows of a tile, a multiple of 16 (32)
   int n_tiles, m_tiles, tiles, k_blocks, stages;
   int splits;                                // CTAs (a cluster) per tile; 0: whole tiles and ranges
   int cut;                                   // the first `cut` tiles are cut into ranges of
@@ -58,13 +66,70 @@ struct Int8Params {
   unsigned int* counters;                    // [CTA], zero when the kernel starts
 };
 
+template <bool PAIR>
 OGB_DEVICE void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
-      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// A pair's barriers.  What both CTAs report (bytes that have landed, accumulators that have been read) is counted by the first one's, which issues the products;
+// what its products report (operands read, sums complete) arrives at the same barrier of both.
+OGB_DEVICE uint32_t i8_pair_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+OGB_DEVICE uint32_t i8_first_addr(const void* p) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+OGB_DEVICE void i8_first_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(i8_first_addr(bar)) : "memory"); }
+OGB_DEVICE bool i8_pair_wait(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t spins = 0;; ++spins) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok != 0) return true;
+    if ((spins & 0x3ff) == 0x3ff && global_timer_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+template <bool PAIR>
+OGB_DEVICE bool i8_wait(uint64_t* bar, uint32_t parity) { return PAIR ? i8_pair_wait(bar, parity) : mbar_wait(bar, parity); }
+template <bool PAIR>
+OGB_DEVICE void i8_commit(uint64_t* bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+  else umma_commit(bar);
+}
+template <bool PAIR>
+OGB_DEVICE void i8_load(void* to, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_u32(to)), "l"(reinterpret_cast<uint64_t>(map)), "r"(i8_first_addr(bar)), "r"(x), "r"(y) : "memory");
+  else tma_load_2d(to, map, bar, x, y);
+}
+OGB_DEVICE void i8_pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // kind::i8: signed 8-bit A and B, both K-major, 32-bit sums that wrap (they never get that far).
 __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
@@ -79,12 +144,13 @@ OGB_DEVICE void i8_tile(const Int8Params& p, int tile, int& nt, int& mt) {
   if (p.m_tiles == 1) {
     nt = tile;
     mt = 0;
-    return;
+  } else {
+    const int g = tile / (kI8Group * p.m_tiles), first = g * kI8Group;
+    const int wide = min(kI8Group, p.n_tiles - first), t = tile - first * p.m_tiles;
+    nt = first + t % wide;
+    mt = t / wide;
   }
-  const int g = tile / (kI8Group * p.m_tiles), first = g * kI8Group;
-  const int wide = min(kI8Group, p.n_tiles - first), t = tile - first * p.m_tiles;
-  nt = first + t % wide;
-  mt = t / wide;
+  if (p.pair != 0) nt = 2 * nt + (blockIdx.x & 1);
 }
 
 OGB_DEVICE int i8_cluster_index() {
@@ -105,7 +171,8 @@ struct Int8Segs {
   int it0, it1, first_end, last_begin, mid;
   int k_blocks, state = 0, tile, tiles, stride;
   OGB_DEVICE explicit Int8Segs(const Int8Params& p) : k_blocks(p.k_blocks), tiles(p.tiles) {
-    stride = gridDim.x;
+    const int unit = blockIdx.x >> p.pair;
+    stride = gridDim.x >> p.pair;
     if (p.splits > 0) {
       state = 3;
       tile = p.splits == 1 ? blockIdx.x : i8_cluster_index();
@@ -114,9 +181,9 @@ struct Int8Segs {
       it1 = i8_range_begin(p, rank + 1);
       return;
     }
-    tile = p.cut + blockIdx.x;
-    it0 = i8_range_begin(p, blockIdx.x);
-    it1 = i8_range_begin(p, blockIdx.x + 1);
+    tile = p.cut + unit;
+    it0 = i8_range_begin(p, unit);
+    it1 = i8_range_begin(p, unit + 1);
     first_end = it0;
     last_begin = it1;
     if (it1 > it0) {
@@ -307,7 +374,7 @@ OGB_DEVICE void i8_group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r
 
 // The epilogue warps, where whole tiles and ranges are computed.  Warp index mod 4: the quarter of TMEM's lanes, 32 channels of a tile; each of the
 // two groups takes every other chunk of rows.
-template <int TW, int OUT>
+template <int TW, int OUT, bool PAIR>
 OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars, int* staging) {
   constexpr int kChunk = kI8Chunk<TW>;
   const int warp = (threadIdx.x >> 5) - 2, q = (threadIdx.x >> 5) & 3, group = warp >> 2, lane = threadIdx.x & 31;
@@ -318,6 +385,10 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
   pdl_wait();
   const float* factor = after_wait(p.factor);
   bool ok = true;
+  // this warp has read an accumulator
+  auto release = [&](int buf) {
+    if (lane == 0) PAIR ? i8_first_arrive(&bars->tmem_empty[buf]) : mbar_arrive(&bars->tmem_empty[buf]);
+  };
   Int8Segs segs(p);
   int tile, kb0, kb1;
   for (int seg = 0; segs.next(tile, kb0, kb1); ++seg) {
@@ -343,7 +414,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     chunk_residual(group * kChunk);
     // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out the warps go on
     // to arrive on the counters of their shared tiles.
-    if (ok && !__all_sync(0xffffffffu, mbar_wait(&bars->tmem_full[buf], buf_phase))) {
+    if (ok && !__all_sync(0xffffffffu, i8_wait<PAIR>(&bars->tmem_full[buf], buf_phase))) {
       ok = false;
       if (lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *abort_flag = 1; }
     }
@@ -371,9 +442,9 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
       tc_fence_before();
       __threadfence();
       i8_epi_sync();
-      if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+      release(buf);
       if (warp == 0 && lane == 0) {
-        *shared_last = atomicAdd(p.counters + c_lo, 1u) == static_cast<unsigned int>(c_hi - c_lo - 1);
+        *shared_last = atomicAdd(p.counters + (PAIR ? 2 * c_lo + (blockIdx.x & 1) : c_lo), 1u) == static_cast<unsigned int>(c_hi - c_lo - 1);
         __threadfence();
       }
       i8_epi_sync();
@@ -406,7 +477,8 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
             for (int i = 0; i < 2; ++i) {
               // the first CTA of a tile holds its head (slot 1), the others a later part (slot 0)
               const int from = min(x + i, c_hi - 1);
-              const int4* src = reinterpret_cast<const int4*>(p.ws + static_cast<size_t>(from * 2 + (from == c_lo ? 1 : 0)) * slot) +
+              const int cta = PAIR ? 2 * from + (blockIdx.x & 1) : from;
+              const int4* src = reinterpret_cast<const int4*>(p.ws + static_cast<size_t>(cta * 2 + (from == c_lo ? 1 : 0)) * slot) +
                                 ((w * 4 + q) * acc_cols + c) * 8 + lane;
 #pragma unroll
               for (int j = 0; j < kChunk / 4; ++j) t[i][j] = __ldcg(src + j * 32);
@@ -442,7 +514,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     if (whole) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->tmem_empty[buf]);
+      release(buf);
     }
   }
 }
@@ -534,9 +606,9 @@ OGB_DEVICE void i8_finish_cluster(const Int8Params& p, uint32_t tmem_base, int a
   if (p.splits > 1) cooperative_groups::this_cluster().sync();
 }
 
-template <int TW>
+template <int TW, bool PAIR>
 OGB_DEVICE bool i8_issue_mma(const Int8Params& p, uint8_t* smem, int stage_bytes, uint32_t tmem_base, int bufs, int acc_cols, RowsBars* bars) {
-  const uint32_t idesc = make_idesc_i8(128, p.mn);
+  const uint32_t idesc = make_idesc_i8(PAIR ? 256 : 128, p.mn);
   int stage = 0;
   uint32_t phase = 0;
   Int8Segs segs(p);
@@ -544,11 +616,11 @@ OGB_DEVICE bool i8_issue_mma(const Int8Params& p, uint8_t* smem, int stage_bytes
   for (int seg = 0; segs.next(tile, kb0, kb1); ++seg) {
     const int buf = bufs == 2 ? (seg & 1) : 0;
     const uint32_t buf_phase = (bufs == 2 ? seg >> 1 : seg) & 1;
-    if (!mbar_wait(&bars->tmem_empty[buf], buf_phase ^ 1)) return false;
+    if (!i8_wait<PAIR>(&bars->tmem_empty[buf], buf_phase ^ 1)) return false;
     tc_fence_after();
     const uint32_t d_addr = tmem_base + buf * TW * acc_cols;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!mbar_wait(&bars->full[stage], phase)) return false;
+      if (!i8_wait<PAIR>(&bars->full[stage], phase)) return false;
       tc_fence_after();
       const uint32_t sw = smem_u32(smem + stage * stage_bytes);
       const uint64_t db = make_kmajor_sw128_desc(sw + TW * 128 * kI8K);
@@ -557,22 +629,23 @@ OGB_DEVICE bool i8_issue_mma(const Int8Params& p, uint8_t* smem, int stage_bytes
         const uint64_t da = make_kmajor_sw128_desc(sw + w * 128 * kI8K);
         // 32 values of K an instruction: +2 in the (>> 4) address field
 #pragma unroll
-        for (int k = 0; k < kI8K / 32; ++k) umma_i8(d_addr + w * acc_cols, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kI8K / 32; ++k) umma_i8<PAIR>(d_addr + w * acc_cols, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
       }
-      umma_commit(&bars->empty[stage]);
+      i8_commit<PAIR>(&bars->empty[stage]);
       if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
-    umma_commit(&bars->tmem_full[buf]);
+    i8_commit<PAIR>(&bars->tmem_full[buf]);
   }
   return true;
 }
 
-template <int TW, int OUT>
+template <int TW, int OUT, bool PAIR>
 __global__ void __launch_bounds__(kI8Threads, 1)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q, const Int8Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   constexpr int kStageW = TW * 128 * kI8K;
-  const int stage_bytes = kStageW + p.mn * kI8K;
+  const int half = PAIR ? p.mn / 2 : p.mn;                     // rows that this CTA brings
+  const int stage_bytes = kStageW + half * kI8K;
   const int ring_bytes = p.stages * stage_bytes;
   RowsBars* bars = reinterpret_cast<RowsBars*>(smem + ring_bytes);
   int* staging = reinterpret_cast<int*>(smem + ring_bytes + kRowsBarBytes);
@@ -584,11 +657,12 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   // The thread that issues the loads makes the barriers, and has the first ring of W on its way before anything else is set up -- and before
   // the kernel ahead, which makes the rows, has ended.
   int ahead = 0;
+  const uint32_t rank = PAIR ? i8_pair_rank() : 0;
   auto load_w = [&](const Int8Cursor& c, int st) {
-    mbar_expect_tx(&bars->full[st], stage_bytes);
+    if (rank == 0) mbar_expect_tx(&bars->full[st], PAIR ? 2 * stage_bytes : stage_bytes);
 #pragma unroll
     for (int w = 0; w < TW; ++w)
-      tma_load_2d(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (c.nt * TW + w) * 128);
+      i8_load<PAIR>(smem + st * stage_bytes + w * 128 * kI8K, &tmap_w, &bars->full[st], c.kb * kI8K, (c.nt * TW + w) * 128);
   };
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
@@ -597,19 +671,27 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->tmem_full[i], 1);
-      mbar_init(&bars->tmem_empty[i], 4 * kI8Groups);
+      mbar_init(&bars->tmem_empty[i], (PAIR ? 2 : 1) * 4 * kI8Groups);
     }
     bars->abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
-    for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
+    if (!PAIR)
+      for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
   }
   if (warp == 1) {
-    tmem_alloc(&bars->tmem_slot, tmem_cols);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      __syncwarp();
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_slot)), "r"(tmem_cols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(&bars->tmem_slot, tmem_cols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) i8_pair_sync();                                    // loads of either CTA report to the first one's barriers
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_slot;
   pdl_trigger();
@@ -620,15 +702,22 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      if (PAIR)
+        for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
       pdl_wait();
       for (Int8Cursor c(p); c.more; c.step()) {
         if (ahead > 0) {
           --ahead;
         } else {
-          if (!mbar_wait(&bars->empty[stage], phase ^ 1)) { ok = false; break; }
+          if (!i8_wait<PAIR>(&bars->empty[stage], phase ^ 1)) { ok = false; break; }
           load_w(c, stage);
         }
-        tma_load_2d(smem + stage * stage_bytes + kStageW, &tmap_q, &bars->full[stage], c.kb * kI8K, c.mt * p.mn);
+        i8_load<PAIR>(smem + stage * stage_bytes + kStageW, &tmap_q, &bars->full[stage], c.kb * kI8K, c.mt * p.mn + static_cast<int>(rank) * half);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      // a CTA stays for what the other one's products still report to it
+      for (int i = 0; PAIR && ok && i < p.stages; ++i) {
+        ok = i8_wait<PAIR>(&bars->empty[stage], phase ^ 1);
         if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
       if (!ok) { atomicOr(p.status, kStatusWaitTimeout); *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1; }
@@ -636,16 +725,33 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------ MMA issuer ------------------------------
-    if (lane == 0 && !i8_issue_mma<TW>(p, smem, stage_bytes, tmem_base, bufs, acc_cols, bars)) {
+    if (lane == 0 && rank == 0 && !i8_issue_mma<TW, PAIR>(p, smem, stage_bytes, tmem_base, bufs, acc_cols, bars)) {
       atomicOr(p.status, kStatusWaitTimeout);
       *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1;
     }
     __syncwarp();
   } else if (p.splits == 0) {
-    i8_epilogue<TW, OUT>(p, tmem_base, bufs, acc_cols, bars, staging);
+    i8_epilogue<TW, OUT, PAIR>(p, tmem_base, bufs, acc_cols, bars, staging);
   }
-  if (p.splits > 0) i8_finish_cluster<TW, OUT>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
-  rows_teardown(bars, tmem_base, tmem_cols);
+  if constexpr (PAIR) {
+    tc_fence_before();
+    __syncthreads();
+    i8_pair_sync();
+    if (*reinterpret_cast<volatile int*>(&bars->abort_flag) != 0 && threadIdx.x == 0) {
+      // a wait ran out: copies that may still be in flight get a bounded time to land
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    __syncthreads();
+    i8_pair_sync();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
+    }
+  } else {
+    if (p.splits > 0) i8_finish_cluster<TW, OUT>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
+    rows_teardown(bars, tmem_base, tmem_cols);
+  }
 }
 
 // ----------------------------------------------------------------------------------------
@@ -837,9 +943,17 @@ static int launch_gemv(const GemvParams& p, cudaStream_t stream) {
 // host side
 // ----------------------------------------------------------------------------------------
 // How a product is divided, from its sizes alone.
+// Two CTAs, an SM each, share the products of 256 channels and 256 rows: each brings its own channels and half of the rows, so that a k-block
+// of 128 x 256 results draws 32 KB through L2 instead of 48, which is what bounds whole tiles (96 bytes a cycle and SM at the tensor cores'
+// rate).  It pays where main loops are long and rounds many, us with pairs and without: 8192 rows, 3584 x 18944 347 and 380, 8192 x 8192 335 and 400; 4096,
+// 4096 x 4096 52 and 56; 600, 37888 x 3584 70 and 74; but 1024, 8192 x 8192, 1.7 rounds, 70 and 66; 4096, 8192 x 1024 53 and 49, where
+// both CTAs' epilogues are waited for.  Gated tiles are no wider for it, having two accumulators each: 2048, 37888 x 3584 240 and 225.
+static bool i8_pairs(int M, int N, int K, bool gated, int sms) {
+  return !gated && M > 256 && K >= 24 * kI8K && static_cast<long long>((N + 255) / 256) * ((M + 255) / 256) >= 3 * (sms / 2);
+}
 struct Int8Plan {
-  int mn, m_tiles, n_tiles, tiles, k_blocks, cut;
-  bool clusters;
+  int mn, m_tiles, n_tiles, tiles, k_blocks, cut, units;
+  bool clusters, pair;
   long long counter_bytes, ws_bytes;
 };
 // The rows of a tile come from an estimate in us: a k-block of a full tile (128 x 256) 0.43 on 148 SMs, of which 0.1 are W's; an epilogue 1 and, over
@@ -848,15 +962,17 @@ struct Int8Plan {
 //   700 rows against 4608 x 3584: four tiles of 176 rows 17.8 us, three of 240 20.4;  1333, 1001 x 2039: 17 of 80 rows 11.6, six of 224 14.1
 //   1000, gated 9728 x 896: eleven of 96 rows 25.6, eight of 128 30.4
 //   ranges: 1500, 3584 x 18944 123 -> 93, 8192 419 -> 401; but 2000, 3584 x 3584 49 -> 62, 4096, 8192 x 8192 193 -> 203
-static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
+static Int8Plan i8_plan(int M, int N, int K, bool gated, int all) {
   Int8Plan r{};
   const int tw = gated ? 2 : 1, most = 256 / tw;
-  r.n_tiles = (N + 128 * tw - 1) / (128 * tw);
+  r.pair = i8_pairs(M, N, K, gated, all);
+  const int sms = r.units = r.pair ? all / 2 : all, wide = r.pair ? 2 : 1;
+  r.n_tiles = (N + 128 * tw * wide - 1) / (128 * tw * wide);
   r.k_blocks = (K + kI8K - 1) / kI8K;
   const int fewest = (M + most - 1) / most;
   float best = 0.f;
   for (int m_tiles = fewest; m_tiles <= fewest + 24; ++m_tiles) {
-    const int mn = ((M + m_tiles - 1) / m_tiles + 15) / 16 * 16;
+    const int mn = ((M + m_tiles - 1) / m_tiles + 16 * wide - 1) / (16 * wide) * (16 * wide);
     const long long tiles = static_cast<long long>(r.n_tiles) * ((M + mn - 1) / mn);
     if (m_tiles > fewest && (tiles > 4 * sms || mn < 32)) break;
     const float part = static_cast<float>(tw * mn) / 256.f, block = 0.1f * tw + 0.33f * part, epilogue = 1.f + 2.f * part;
@@ -880,25 +996,25 @@ static Int8Plan i8_plan(int M, int N, int K, bool gated, int sms) {
     }
   }
   r.tiles = r.m_tiles * r.n_tiles;
-  r.clusters = r.tiles <= sms;
+  r.clusters = !r.pair && r.tiles <= sms;
   if (r.cut > 0) {
-    r.counter_bytes = (static_cast<long long>(sms) * 4 + 1023) / 1024 * 1024;
-    r.ws_bytes = 2ll * sms * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
+    r.counter_bytes = (static_cast<long long>(all) * 4 + 1023) / 1024 * 1024;
+    r.ws_bytes = 2ll * all * tw * 128 * ((r.mn + 31) / 32 * 32) * 4;
   }
   return r;
 }
 
-template <int TW, int OUT>
+template <int TW, int OUT, bool PAIR>
 static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long long ldq, const void* w, long long ldw, int K, bool early, cudaStream_t stream) {
-  auto kernel = gemm_int8_kernel<TW, OUT>;
+  auto kernel = gemm_int8_kernel<TW, OUT, PAIR>;
   static OncePerDevice allowed;
   int rc = allow_smem(allowed, kernel, kRowsSmemMax);
   if (rc != 0) return rc;
-  const int stage_bytes = TW * 128 * kI8K + p.mn * kI8K;
+  const int rows = PAIR ? p.mn / 2 : p.mn, stage_bytes = TW * 128 * kI8K + rows * kI8K;
   const int extra = kRowsBarBytes + (plan.clusters ? 0 : kI8Groups * kI8Stage);
   p.stages = std::min(kRowsMaxStages, (kRowsSmemMax - extra) / stage_bytes);
   const int smem = p.stages * stage_bytes + extra;
-  int grid = ogb_num_sms();
+  int grid = PAIR ? 2 * plan.units : plan.units;
   if (plan.clusters) {
     p.splits = rows_pick_splits(kernel, kI8Threads, smem, p.tiles, p.k_blocks);
     p.range = p.k_blocks / p.splits;
@@ -908,7 +1024,7 @@ static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long l
   CUtensorMap mw, mq;
   rc = make_tmap_u8_2d(&mw, w, p.N, K, ldw, 128, kI8K);
   if (rc != 0) return rc;
-  rc = make_tmap_u8_2d(&mq, q, p.M, K, ldq, p.mn, kI8K);
+  rc = make_tmap_u8_2d(&mq, q, p.M, K, ldq, rows, kI8K);
   if (rc != 0) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -917,9 +1033,9 @@ static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long l
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  if (p.splits > 1) {
+  if (PAIR || p.splits > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = p.splits;
+    attr[cfg.numAttrs].val.clusterDim.x = PAIR ? 2 : p.splits;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
@@ -991,15 +1107,16 @@ extern "C" int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void*
   p.vec = (reinterpret_cast<uintptr_t>(out) % piece == 0 && ldc % 4 == 0 &&
            (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) % piece == 0 && ldr % 4 == 0))) ? 1 : 0;
   p.M = M; p.N = N; p.mn = plan.mn; p.n_tiles = plan.n_tiles; p.m_tiles = plan.m_tiles; p.tiles = plan.tiles; p.k_blocks = plan.k_blocks;
-  p.cut = plan.cut; p.range = plan.cut * plan.k_blocks / sms; p.longer = plan.cut * plan.k_blocks % sms; p.status = status;
-  if (gated != 0) {
-    if (out_elem == kElemF32) return launch_int8<2, kElemF32>(plan, p, q, ldq, w, ldw, K, early, stream);
-    if (out_elem == kElemBf16) return launch_int8<2, kElemBf16>(plan, p, q, ldq, w, ldw, K, early, stream);
-    return launch_int8<2, kElemF16>(plan, p, q, ldq, w, ldw, K, early, stream);
-  }
-  if (out_elem == kElemF32) return launch_int8<1, kElemF32>(plan, p, q, ldq, w, ldw, K, early, stream);
-  if (out_elem == kElemBf16) return launch_int8<1, kElemBf16>(plan, p, q, ldq, w, ldw, K, early, stream);
-  return launch_int8<1, kElemF16>(plan, p, q, ldq, w, ldw, K, early, stream);
+  p.pair = plan.pair ? 1 : 0;
+  p.cut = plan.cut; p.range = plan.cut * plan.k_blocks / plan.units; p.longer = plan.cut * plan.k_blocks % plan.units; p.status = status;
+  auto launch = [&](auto out_type) {
+    constexpr int E = decltype(out_type)::value;
+    if (gated != 0) return launch_int8<2, E, false>(plan, p, q, ldq, w, ldw, K, early, stream);
+    return plan.pair ? launch_int8<1, E, true>(plan, p, q, ldq, w, ldw, K, early, stream) : launch_int8<1, E, false>(plan, p, q, ldq, w, ldw, K, early, stream);
+  };
+  if (out_elem == kElemF32) return launch(std::integral_constant<int, kElemF32>());
+  if (out_elem == kElemBf16) return launch(std::integral_constant<int, kElemBf16>());
+  return launch(std::integral_constant<int, kElemF16>());
 }
 
 // The same call with its arguments as 64-bit words in their order: a binding that converts every argument by itself spends as long on these as on a

@@ -290,13 +290,17 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
                 _refuse("rows of out overlap")
     # a matrix that is written may stand in the place of one that is read, row for row; any other meeting would change what is still to be read
     x_ptr = x.data_ptr()
-    wide, y_wide, gate_wide = (4 if k == 0 else 2 for k in (kind, y_kind, gate_kind))
-    reads = (x_ptr, ldx, kind, wide), (y_ptr, ldy, y_kind, y_wide), (gate_ptr if ldg else 0, ldg, gate_kind, gate_wide)
+    wide = 2 if kind else 4
+    reads = [(x_ptr, ldx, kind, wide)]
+    if y_ptr:
+        reads.append((y_ptr, ldy, y_kind, 2 if y_kind else 4))
+    if ldg:
+        reads.append((gate_ptr, ldg, gate_kind, 2 if gate_kind else 4))
     if new_ptr:
         _separate(new_ptr, ldn, kind, wide, reads, rows, n)
     if out is not None:
         out_kind, out_ptr = ELEM[out_dtype], out.data_ptr()
-        out_wide = 4 if out_kind == 0 else 2
+        out_wide = 2 if out_kind else 4
         _separate(out_ptr, ldo, out_kind, out_wide, reads, rows, n)
         if new_ptr and _meet(new_ptr, rows, ldn * wide, n * wide, out_ptr, rows, ldo * out_wide, n * out_wide):
             _refuse("the new stream and out share memory")
@@ -338,17 +342,19 @@ def block_norm(x, y=None, post=None, gate=None, pre=None, eps=1e-6, x_scale=1.0,
 def _separate(ptr, ld, kind, wide, reads, rows, n):
     end = ptr + ((rows - 1) * ld + n) * wide
     for other, ldr, other_kind, other_wide in reads:
-        if other < end and ptr < other + ((rows - 1) * ldr + n) * other_wide and _meet(ptr, rows, ld * wide, n * wide, other, rows, ldr * other_wide, n * other_wide):
-            if ptr != other or kind != other_kind or (ld != ldr and rows > 1):
+        if other < end and ptr < other + ((rows - 1) * ldr + n) * other_wide:
+            same = ptr == other and kind == other_kind and (ld == ldr or rows == 1)
+            if not same and _meet(ptr, rows, ld * wide, n * wide, other, rows, ldr * other_wide, n * other_wide):
                 _refuse("x_out (or x) and out: matrices that share memory with none, or the very ones that are read")
 
 
 def _matrix(t, shape, dev):
     """Stride of the rows of a matrix that goes with x."""
-    ld, step = t.stride() if t.dim() == 2 else (0, 0)
-    if t.shape != shape or t.dtype not in ELEM or t.device != dev or (step != 1 and shape[1] > 1):
-        _refuse("x, y, x_out, out and a gate for each token: matrices of one shape, fp32, bf16 or fp16, on one device, with neighbouring columns")
-    return ld
+    if t.shape == shape and t.dtype in ELEM and t.device == dev:
+        ld, step = t.stride()
+        if step == 1 or shape[1] == 1:
+            return ld
+    _refuse("x, y, x_out, out and a gate for each token: matrices of one shape, fp32, bf16 or fp16, on one device, with neighbouring columns")
 
 
 def _vector(t, n, dev):
