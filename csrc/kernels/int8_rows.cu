@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, V < kVec ? norm_blocks(V, T
 
 // Eight floats as one store: a whole sector.
 OGB_DEVICE void store32(float* to, const float (&f)[8]) {
-  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),
+  asm volatile("st.global.L1::no_allocate.L2::evict_first.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),
                "f"(f[6]), "f"(f[7])
                : "memory");
 }
@@ -352,7 +352,12 @@ __global__ void __launch_bounds__(T == 32 ? 128 : T, norm_blocks(V, T)) block_no
   const int words = V * (kX + (has_y ? kY : 0) + (gate_row ? kY : 0));
   uint4* mine = slots + threadIdx.x - lane;                                    // the warp's words
   const uint32_t base = smem_u32(mine);
-  auto copy = [](uint32_t to, const char* s) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(s) : "memory"); };
+  // (read once: first to leave L2)
+  uint64_t once;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
+  auto copy = [&](uint32_t to, const char* s) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(s), "l"(once) : "memory");
+  };
   // A warp's 32 pieces of a matrix: 32 words, or of 32-bit values 64.  Lanes copy neighbouring words, so that no 32-byte sector is asked for twice, and
   // take two each from shared memory, where words trade places in every other eight to keep eight lanes on different banks.
   auto fetch_matrix = [&](auto bytes, uint32_t to, const char* s, size_t at, int shift) {
@@ -537,7 +542,8 @@ static int launch_norm_kernel(OncePerDevice& allowed, Kernel kernel, BlockNormPa
   auto words = [](const void* m, int elem) { return m == nullptr ? 0 : elem == kElemF32 ? 2 : 1; };
   const int block = T == 32 ? 128 : threads;
   const int stage = 16 * block * V * (words(p.x, p.x_elem) + words(p.y, p.y_elem) + (p.ldg != 0 ? words(p.gate, p.gate_elem) : 0));
-  const int most = std::max(1, 65536 / ((V < kVec ? 64 : 80) * block));
+  // as many blocks as registers hold: the compiler's 56 a thread with up to two pieces are fewer than the kernel's bound
+  const int most = std::max(1, 65536 / ((V < kVec ? 56 : 80) * block));
   const int exchange = p.q != nullptr && p.shifted != 0 ? (8 * (T == 32 ? 4 * (32 * V + 1) : V * block + 1) + 15) / 16 * 16 : 0;
   const int smem = stage + exchange;
   const int per_sm = std::max(1, std::min(kNormSmem / (smem + 1024), most));

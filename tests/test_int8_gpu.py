@@ -348,3 +348,17 @@ def test_long_k_and_tiles_that_are_cut_into_ranges(m, n, k, gated, cut):
     assert (int8._workspace(m, n, k, gated, False) > 0) is cut
     _check_product(_gen(m + n), m, n, k, BF16, True, not gated, gated)
     _check_product(_gen(m + k), m, n, k, F16, True, False, gated, as_rows=True)
+
+
+@pytest.mark.parametrize("m,n,k,dtype,bias,residual", [(4100, 4001, 4096, F32, False, True), (300, 29000, 3100, BF16, True, False), (1025, 11008, 4097, F16, True, True)])
+def test_long_products_of_many_tiles(m, n, k, dtype, bias, residual):
+    g = _gen(m)
+    _check_product(g, m, n, k, dtype, bias, residual, False)
+    x, (w, c) = _rows(g, m, k, dtype), _weight(g, n, k)
+    res = _rand(g, m, n).to(dtype) if residual else None
+    whole = int8.gemm_int8(x, w, c, residual=res)
+    parts = [int8.gemm_int8(x[i:i + 160], w, c, residual=None if res is None else res[i:i + 160]) for i in range(0, m, 160)]
+    assert torch.equal(whole, torch.cat(parts))            # divided in another way: whole numbers add up to the same
+    buf = torch.full((m + 1, n + 8), 7.0, device="cuda", dtype=dtype)
+    int8.gemm_int8(x, w, c, residual=res, out=buf[:m, :n])
+    assert torch.equal(buf[:m, :n], whole) and bool((buf[m] == 7.0).all()) and bool((buf[:, n:] == 7.0).all())
