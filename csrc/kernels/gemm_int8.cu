@@ -128,9 +128,7 @@ OGB_DEVICE void i8_load(void* to, const CUtensorMap* map, uint64_t* bar, int x, 
                  ::"r"(smem_u32(to)), "l"(reinterpret_cast<uint64_t>(map)), "r"(i8_first_addr(bar)), "r"(x), "r"(y) : "memory");
   else tma_load_2d(to, map, bar, x, y);
 }
-OGB_DEVICE void i8_pair_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+OGB_DEVICE void i8_pair_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 // kind::i8: signed 8-bit A and B, both K-major, 32-bit sums that wrap (they never get that far).
 __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
   return (2u << 4)                      // D format: s32
@@ -679,6 +677,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     if (!PAIR)
       for (Int8Cursor c(p); c.more && ahead < p.stages; c.step()) load_w(c, ahead++);
   }
+  if constexpr (PAIR) i8_pair_sync();                          // both CTAs run: tensor memory is allocated on both SMs, and loads of either report to the first one's barriers
   if (warp == 1) {
     if constexpr (PAIR) {
       __syncwarp();
@@ -691,7 +690,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (PAIR) i8_pair_sync();                                    // loads of either CTA report to the first one's barriers
+  if constexpr (PAIR) i8_pair_sync();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_slot;
   pdl_trigger();
@@ -746,8 +745,10 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     i8_pair_sync();
     if (warp == 1) {
       tc_fence_after();
+      __syncwarp();
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
     }
+    i8_pair_sync();                                            // neither leaves before the other has given its share back
   } else {
     if (p.splits > 0) i8_finish_cluster<TW, OUT>(p, tmem_base, acc_cols, bars, smem, ring_bytes);
     rows_teardown(bars, tmem_base, tmem_cols);
@@ -1039,7 +1040,7 @@ static int launch_int8(const Int8Plan& plan, Int8Params p, const void* q, long l
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
-  if (early) {
+  if (early && !PAIR) {      // a pair starts when the kernel ahead has ended: it needs two SMs at once, and is long
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
