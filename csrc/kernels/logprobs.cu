@@ -17,6 +17,8 @@
 //
 // A row is split over a cluster of CTAs where rows are few; the parts join over distributed shared memory.
 //
+// Measured, bf16: 3500 rows of 152064 170 us (6.2 TB/s), with entropies 192, with these and the 20 likeliest 239; 256 rows 21 and 30; one row 8.
+//
 // Logits may be minus infinity (masked): they weigh nothing.  A row of them has NaN for log probability and entropy, as a row that holds a NaN
 // or plus infinity has; among the likeliest NaN comes last.
 #include <cooperative_groups.h>
@@ -199,6 +201,7 @@ OGB_DEVICE int lp_place(const unsigned long long* keys, int n, unsigned long lon
   return above;
 }
 
+// Read once, so first to leave L2 (256 rows: 21.6 us without that, 20.9 with it).
 // The piece of a row of `vocab` logits that begins at value i0 (below zero or past the end where the row's ends are not at multiples of 32 bytes).
 template <typename T>
 OGB_DEVICE void lp_load(const T* x, int i0, int vocab, uint32_t (&w)[8]) {
