@@ -362,3 +362,26 @@ def test_long_products_of_many_tiles(m, n, k, dtype, bias, residual):
     buf = torch.full((m + 1, n + 8), 7.0, device="cuda", dtype=dtype)
     int8.gemm_int8(x, w, c, residual=res, out=buf[:m, :n])
     assert torch.equal(buf[:m, :n], whole) and bool((buf[m] == 7.0).all()) and bool((buf[:, n:] == 7.0).all())
+
+
+def test_long_products_on_two_streams_and_replayed():
+    g = _gen(5)
+    x, (w, c) = _rows(g, 700, 3200, BF16), _weight(g, 19200, 3200)
+    want = int8.gemm_int8(x, w, c)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(int8.gemm_int8(x, w, c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, t) for t in got)
+    graph, y = torch.cuda.CUDAGraph(), torch.empty_like(want)
+    with torch.cuda.graph(graph):
+        int8.gemm_int8(x, w, c, out=y)
+    for i in range(2):
+        x.mul_(-1.0)
+        y.zero_()
+        graph.replay()
+        assert torch.equal(y, -want if i == 0 else want)
+    ops.check_status()
