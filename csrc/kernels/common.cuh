@@ -97,6 +97,21 @@ OGB_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns = kW
   return true;
 }
 
+// Whether `v` holds in all of the `threads` threads (whole, converged warps) that meet at named barrier `id`.  Where a bounded wait decides whether warps take
+// a path with barriers of their own, they decide together: one that went another way alone would leave the others in them for good.
+OGB_DEVICE bool barrier_all(int id, int threads, bool v) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(all)
+      : "r"(v ? 1u : 0u), "r"(id), "r"(threads)
+      : "memory");
+  return all != 0;
+}
+
 // ----------------------------------------------------------------------------------------
 // TMA (tiled tensor copies; never cluster-multicast)
 // ----------------------------------------------------------------------------------------

@@ -369,6 +369,7 @@ OGB_DEVICE void i8_tmem_ld(uint32_t addr, uint32_t (&r)[kI8Chunk<TW>]) {
 // Barriers of the epilogue warps: all of them, or a group's.
 OGB_DEVICE void i8_epi_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 OGB_DEVICE void i8_group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(2 + group) : "memory"); }
+OGB_DEVICE bool i8_group_all(int group, bool v) { return barrier_all(2 + group, 128, v); }
 
 // The epilogue warps, where whole tiles and ranges are computed.  Warp index mod 4: the quarter of TMEM's lanes, 32 channels of a tile; each of the
 // two groups takes every other chunk of rows.
@@ -410,9 +411,9 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
     };
     float f = chunk_factor(group * kChunk);
     chunk_residual(group * kChunk);
-    // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out the warps go on
-    // to arrive on the counters of their shared tiles.
-    if (ok && !__all_sync(0xffffffffu, i8_wait<PAIR>(&bars->tmem_full[buf], buf_phase))) {
+    // Every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  Each warp's wait has a clock of its own, so the warps
+    // of a group settle together whether it ended (specs/epilogue_votes.py).  After one that ran out they go on to arrive on the counters of their shared tiles.
+    if (ok && !i8_group_all(group, __all_sync(0xffffffffu, i8_wait<PAIR>(&bars->tmem_full[buf], buf_phase)))) {
       ok = false;
       if (lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *abort_flag = 1; }
     }
@@ -448,7 +449,7 @@ OGB_DEVICE void i8_epilogue(const Int8Params& p, uint32_t tmem_base, int bufs, i
       i8_epi_sync();
       const bool last = *shared_last != 0;
       i8_epi_sync();
-      if (!__all_sync(0xffffffffu, ok && last)) continue;
+      if (!__all_sync(0xffffffffu, ok && last)) continue;     // both alike in all warps of the group
     } else if (!ok) {
       continue;
     }

@@ -1,0 +1,37 @@
+"""Bounded waits in front of barriers that only some warps reach: a wait that runs out in one warp never leaves another behind."""
+import os
+import re
+
+import pytest
+
+from onnx_genai_b200.specs import epilogue_votes
+
+KERNELS = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc", "kernels")
+
+
+@pytest.mark.parametrize("warps,tiles,barriers", [(2, 1, 1), (2, 3, 2), (4, 2, 2), (3, 2, 4)])
+def test_warps_that_decide_together_all_reach_the_end(warps, tiles, barriers):
+    r = epilogue_votes.check(warps, tiles, barriers)
+    assert r.ok and r.states > 10, str(r)
+
+
+def test_a_warp_that_decides_alone_leaves_the_others_in_the_groups_barrier():
+    r = epilogue_votes.check(2, 1, 1, vote=False)
+    assert not r.ok and r.kind == "deadlock" and any("gives up" in s for s in r.trace) and any("sees" in s for s in r.trace), str(r)
+
+
+def _body(path, name):
+    """The function's text, from its name to the line that closes it."""
+    with open(os.path.join(KERNELS, path), encoding="utf-8") as f:
+        text = f.read()
+    start = re.search(r"^OGB_DEVICE void %s\(" % name, text, flags=re.M).start()
+    return text[start:text.index("\n}\n", start)]
+
+
+@pytest.mark.parametrize("path,name,vote", [("gemm_int8.cu", "i8_epilogue", "i8_group_all(")])
+def test_the_epilogues_vote_before_any_warp_leaves_a_tile(path, name, vote):
+    body = _body(path, name)
+    wait = body.index("&bars->tmem_full[buf]" if "&bars->tmem_full[buf]" in body else "&tmem_full[buf]")
+    line = body[body.rindex("\n", 0, wait):body.index("\n", wait)]
+    assert vote in line, "each warp goes by its own wait:" + line
+    assert "continue;" not in body[:wait]
