@@ -204,6 +204,7 @@ OGB_DEVICE void rows_store(const RowsGemmParams& p, const ActArgs& act, int m, i
   }
 }
 OGB_DEVICE void rows_epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+OGB_DEVICE bool rows_epi_all(bool v) { return barrier_all(1, 128, v); }
 
 // Ranges: the four epilogue warps (warp index mod 4 = TMEM lane quarter = columns 32 q .. 32 q + 31 of a tile).  stage: TW * kRowsStage
 // bytes, shared_last: one word.
@@ -223,9 +224,10 @@ OGB_DEVICE void rows_epilogue(const RowsGemmParams& p, const ActArgs& act, uint3
     const bool head = kb0 == 0, whole = head && kb1 == k_blocks;
     const int buf = bufs == 2 ? (seg & 1) : 0;
     const uint32_t buf_phase = (bufs == 2 ? seg >> 1 : seg) & 1;
-    // every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  After a wait that ran out
-    // the warps go on to arrive on the counters of their shared tiles, so that they still wrap to zero.
-    if (ok && !__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], buf_phase))) {
+    // Every lane polls (each needs the acquire); the vote keeps the warp converged for tcgen05.ld.  Each warp's wait has a clock of its own, so the four
+    // settle together whether it ended (specs/epilogue_votes.py).  After one that ran out they go on to arrive on the counters of their
+    // shared tiles, so that they still wrap to zero.
+    if (ok && !rows_epi_all(__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], buf_phase)))) {
       ok = false;
       if (lane == 0) { atomicOr(p.status, kStatusWaitTimeout); *abort_flag = 1; }
     }
@@ -263,7 +265,7 @@ OGB_DEVICE void rows_epilogue(const RowsGemmParams& p, const ActArgs& act, uint3
       rows_epi_sync();
       const bool last = *shared_last != 0;
       rows_epi_sync();
-      if (!__all_sync(0xffffffffu, ok && last)) continue;
+      if (!__all_sync(0xffffffffu, ok && last)) continue;     // both alike in all four warps
     } else if (!ok) {
       continue;
     }

@@ -28,7 +28,7 @@ def _body(path, name):
     return text[start:text.index("\n}\n", start)]
 
 
-@pytest.mark.parametrize("path,name,vote", [("gemm_int8.cu", "i8_epilogue", "i8_group_all(")])
+@pytest.mark.parametrize("path,name,vote", [("gemm_int8.cu", "i8_epilogue", "i8_group_all("), ("gemm_rows.cuh", "rows_epilogue", "rows_epi_all(")])
 def test_the_epilogues_vote_before_any_warp_leaves_a_tile(path, name, vote):
     body = _body(path, name)
     wait = body.index("&bars->tmem_full[buf]" if "&bars->tmem_full[buf]" in body else "&tmem_full[buf]")
