@@ -332,7 +332,7 @@ class LLMEngine:
         itself, a step's worth of rows at a time (``max_logit_rows``): no request may be in flight."""
         if self.tp > 1 or self.pp > 1:
             raise ValueError("score() runs on one GPU")
-        if self.has_work or self.stats or self.forced:
+        if self.has_work or self.forced:         # (figures of requests that are over may stay: generate() keeps them)
             raise RuntimeError("score() drives the engine by itself: finish the requests in flight first")
         rows = self.logit_row_limit
         empty = ops.token_logprobs(torch.zeros(0, self.cfg.model.vocab), torch.zeros(0, dtype=torch.int32), top, entropy)      # refuses what a step would
