@@ -314,9 +314,10 @@ void Core::publish_full_pages(Sequence& s) {
 
 void Core::try_prefix_attach(Sequence& s) {
   if (!cfg_.enable_prefix_cache || !s.pages.empty()) return;
-  if (s.forced && !s.wanted.empty()) return;               // its logits rows come from computing the positions, cached or not
   // never serve the whole prompt from cache: the last token must run to produce logits
-  const int max_full = (static_cast<int>(s.tokens.size()) - 1) / kPageTokens;
+  int max_full = (static_cast<int>(s.tokens.size()) - 1) / kPageTokens;
+  // a forced sequence's logits rows come from computing their positions: only what lies ahead of the first may be cached
+  if (s.forced && !s.wanted.empty()) max_full = std::min(max_full, s.wanted.front() / kPageTokens);
   uint64_t h = 0;
   int matched = 0;
   for (int i = 0; i < max_full; ++i) {

@@ -39,3 +39,39 @@ def test_an_engine_scores_after_it_has_generated():
     eng.add_request([1, 2, 3], 2)
     with pytest.raises(RuntimeError):
         eng.score([tokens])
+
+
+def _forced(eng, tokens, want):
+    """Rows of the wanted places, and how many tokens the engine computed for them."""
+    sid = eng.open_forced(tokens, want)
+    rows, computed = [], 0
+    while eng.forced_pending(sid) > 0:
+        out = eng.step()
+        rows += out.forced_logits.get(sid, [])
+        computed += out.num_tokens
+    eng.close_forced(sid)
+    assert [p for p, _ in rows] == list(want)
+    return torch.stack([r for _, r in rows]), computed
+
+
+@pytest.mark.parametrize("first,cached", [(0, 0), (15, 0), (16, 16), (47, 32), (48, 48), (63, 48), (89, 80)])
+def test_forced_rows_take_from_the_prefix_cache_what_lies_ahead_of_them(first, cached):
+    tokens = _tokens(90, 3)
+    want = list(range(first, 90, 17)) + ([89] if (89 - first) % 17 else [])
+    fresh, all_of_it = _forced(_engine(max_logit_rows=90, enable_prefix_cache=False), tokens, want)
+    eng = _engine(max_logit_rows=90)
+    _, computed = _forced(eng, tokens, [89])
+    assert computed == all_of_it == 90
+    rows, computed = _forced(eng, tokens, want)
+    assert computed == 90 - cached
+    torch.testing.assert_close(rows, fresh, rtol=0, atol=1e-4)
+
+
+def test_scores_of_texts_that_share_a_prefix():
+    shared = _tokens(50, 4)
+    texts = [shared + _tokens(n, 5 + n) for n in (3, 30, 1)] + [shared]
+    eng = _engine()
+    for text, r in zip(texts, eng.score(texts, top=2, entropy=True)):
+        want, = _engine(enable_prefix_cache=False).score([text], top=2, entropy=True)
+        torch.testing.assert_close(r.logprob, want.logprob, rtol=0, atol=1e-5)
+        assert torch.equal(r.top_ids, want.top_ids)
