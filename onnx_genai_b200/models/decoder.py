@@ -73,7 +73,8 @@ def pad_mlp(gate, up, down, multiple: int = 64):
 
 def quantize_int8(weights: DecoderWeights) -> DecoderWeights:
     """Turns the layers' matrices into 8-bit weights with a factor per channel, in place and one layer at a time; their products quantise
-    activations a token at a time (ops.int8).  Embeddings, norms and the LM head stay as they are.  For dense layers on one GPU."""
+    activations a token at a time (ops.int8).  Embeddings, norms and the LM head stay as they are.  For dense layers on one GPU; weights that are
+    refused stay as they are."""
     from ..ops import int8
 
     half = weights.swiglu_half
@@ -82,6 +83,11 @@ def quantize_int8(weights: DecoderWeights) -> DecoderWeights:
             continue
         if l.quant or l.router_w is not None or l.gate_up_w is None:
             raise ValueError(f"layer {i} has {'int4' if l.quant else 'expert'} weights: 8-bit weights are made of dense ones")
+        if not all(bool(torch.isfinite(w).all()) for w in (l.qkv_w, l.o_w, l.gate_up_w, l.down_w)):
+            raise ValueError(f"layer {i} has weights that are not finite: they cannot be held in 8 bits")
+    for l in weights.layers:
+        if l.int8:
+            continue
         w = l.gate_up_w
         blocks = w.view(-1, 2, half, w.shape[1])
         gate_up = int8.quantize_gate_up(blocks[:, 0].reshape(-1, w.shape[1]), blocks[:, 1].reshape(-1, w.shape[1]))

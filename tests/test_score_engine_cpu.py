@@ -5,7 +5,7 @@ import torch
 
 from onnx_genai_b200.engine.llm_engine import EngineConfig, LLMEngine
 from onnx_genai_b200.models.config import DecoderConfig
-from onnx_genai_b200.models.decoder import random_weights
+from onnx_genai_b200.models.decoder import quantize_int8, random_weights
 
 CFG = DecoderConfig(name="t", num_layers=2, hidden=64, num_heads=4, num_kv_heads=2, head_dim=16, intermediate=96, vocab=300,
                     rope_theta=1e4, tie_embeddings=True, qkv_bias=True, max_position=512)
@@ -75,3 +75,20 @@ def test_scores_of_texts_that_share_a_prefix():
         want, = _engine(enable_prefix_cache=False).score([text], top=2, entropy=True)
         torch.testing.assert_close(r.logprob, want.logprob, rtol=0, atol=1e-5)
         assert torch.equal(r.top_ids, want.top_ids)
+
+
+@pytest.mark.parametrize("bad", ["int4", "experts", "infinite"])
+def test_weights_that_cannot_be_held_in_8_bits_stay_as_they_are(bad):
+    w = _weights()
+    last = w.layers[1]
+    if bad == "int4":
+        last.quant = {"o": None}
+    elif bad == "experts":
+        last.router_w = torch.zeros(4, CFG.hidden)
+    else:
+        last.down_w[3, 5] = float("inf")
+    keep = [(l.qkv_w, l.qkv_b, l.o_w, l.gate_up_w, l.down_w) for l in w.layers]
+    with pytest.raises(ValueError, match="layer 1"):
+        quantize_int8(w)
+    for l, was in zip(w.layers, keep):
+        assert not l.int8 and all(a is b for a, b in zip((l.qkv_w, l.qkv_b, l.o_w, l.gate_up_w, l.down_w), was))
