@@ -128,6 +128,8 @@ class LLMEngine:
             if not isinstance(weights, DecoderWeights) or tp > 1 or self.pp > 1 or cfg.weight_offload_layers or cfg.compute_dtype != "bf16":
                 raise ValueError("8-bit weights are made for dense bf16 decoders on one GPU, without weight offload")
             quantize_int8(weights)
+            if is_cuda:
+                torch.cuda.empty_cache()         # the matrices' old memory counts as taken, and would be missing from the pool of pages
         self.weights = weights
         max_pages_per_seq = (cfg.max_seq_len + ops.PAGE - 1) // ops.PAGE
         hs = shard_heads(m.num_heads, m.num_kv_heads, tp, shard_rank)
