@@ -566,8 +566,19 @@ def _save_png(path: str, chw) -> None:
         f.write(encode_png(chw))
 
 
+def _json_values(v):
+    """``v`` with None in the place of infinities and NaN, for which JSON has no number."""
+    if isinstance(v, dict):
+        return {k: _json_values(x) for k, x in v.items()}
+    if isinstance(v, (list, tuple)):
+        return [_json_values(x) for x in v]
+    return None if isinstance(v, float) and not math.isfinite(v) else v
+
+
 def cmd_score(args, profiler):
-    """Log probabilities of given texts under the model, a JSON line each, and the perplexity of all of them together."""
+    """Log probabilities of given texts under the model, a JSON line each (null for what is infinite), and the perplexity of all of them together."""
+    from .engine.api import perplexity
+
     eng = _load(args)
     if eng.tokenizer is None and not args.ids:
         print("score: this model directory has no tokenizer.json; give token ids, with --ids", file=sys.stderr)
@@ -581,10 +592,10 @@ def cmd_score(args, profiler):
         return 2
     total, count = 0.0, 0
     for doc in docs:
-        print(json.dumps(doc))
+        print(json.dumps(_json_values(doc), allow_nan=False))
         total, count = total + sum(doc["logprobs"]), count + len(doc["logprobs"])
     if count:
-        print(f"{len(docs)} texts, {count} tokens scored, perplexity {math.exp(-total / count):.4f}", file=sys.stderr)
+        print(f"{len(docs)} texts, {count} tokens scored, perplexity {perplexity(total / count):.4f}", file=sys.stderr)
     return 0
 
 

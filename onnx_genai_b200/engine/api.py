@@ -9,6 +9,7 @@ checkpoint / restore / rewind / fork (runtime.rs:1240-1330, config.rs:472-484).
 """
 from __future__ import annotations
 
+import math
 import os
 
 import time
@@ -89,6 +90,14 @@ class GenerateResult:
     def decode_tokens_per_s(self) -> float:
         dt = self.total_s - self.ttft_s
         return (self.completion_tokens - 1) / dt if dt > 0 and self.completion_tokens > 1 else 0.0
+
+
+def perplexity(mean_logprob: float) -> float:
+    """exp(-mean); infinite where that is past the range of a float (a mean below -709)."""
+    try:
+        return math.exp(-mean_logprob)
+    except OverflowError:
+        return math.inf
 
 
 @dataclass
@@ -323,7 +332,7 @@ class Engine:
         for tokens, r in zip(ids, self.llm.score(ids, top=top, entropy=True)):
             n = len(tokens) - 1
             doc = {"token_ids": tokens, "logprobs": r.logprob.tolist(), "ranks": r.rank.tolist(), "entropies": r.entropy.tolist(),
-                   "perplexity": float(np.exp(-float(r.logprob.double().mean()))) if n else None}
+                   "perplexity": perplexity(float(r.logprob.double().mean())) if n else None}
             if top:
                 doc["top"] = [list(zip(i, v)) for i, v in zip(r.top_ids.tolist(), r.top_logprobs.tolist())]
             out.append(doc)
