@@ -520,7 +520,7 @@ extern "C" int ogb_token_logprobs(const void* logits, const int* tokens, float* 
   if (rows < 0 || vocab < 1 || ld < 0 || elem < 0 || elem >= kElemKinds) return -2;
   if (top < 0 || top > kLpMaxTop || top > vocab || (rows > 0 && top > 0 && (top_ids == nullptr || top_logprob == nullptr))) return -3;
   if (rows == 0) return 0;
-  if (vocab > (1 << 30) || rows > (1 << 28)) return -2;
+  if (vocab > (1 << 30) || rows >= (1 << 28)) return -2;      // a grid of up to kLpMaxSplit CTAs a row has 31 bits
   LogprobsParams p{logits, tokens, logprob, entropy, top_logprob, rank, top_ids, ld, rows, vocab, top, 1, status};
   const int sms = ogb_num_sms();
   // parts of a row: until every SM has a few CTAs, as long as each keeps a piece or so a thread; more where the maxima of its pieces would not fit

@@ -564,6 +564,7 @@ _TOKEN_TYPES = (torch.int32, torch.int64)
 _pack_logprobs = struct.Struct("14q").pack      # a call with its arguments in one word: ctypes converts them one by one else
 MAX_TOP_LOGPROBS = 32
 MAX_VOCAB, MAX_VOCAB_WITH_TOP = 1 << 30, 3_000_000
+MAX_LOGPROB_ROWS = (1 << 28) - 1                # a grid counts up to eight CTAs a row in 31 bits
 
 
 @_timed("token_logprobs")
@@ -581,8 +582,8 @@ def token_logprobs(logits, tokens, top=0, entropy=False) -> TokenLogprobs:
     rows, vocab = shape
     if not 0 <= top <= (MAX_TOP_LOGPROBS if vocab > MAX_TOP_LOGPROBS else vocab):
         raise ValueError(f"top = {top}: between 0 and {min(MAX_TOP_LOGPROBS, vocab)}")
-    if rows > 1 << 30:
-        raise ValueError(f"{rows} rows: at most {1 << 30}")
+    if rows > MAX_LOGPROB_ROWS:
+        raise ValueError(f"{rows} rows: at most {MAX_LOGPROB_ROWS}")
     if vocab > MAX_VOCAB_WITH_TOP and (top or vocab > MAX_VOCAB):
         raise ValueError(f"a vocabulary of {vocab}: at most {MAX_VOCAB_WITH_TOP if top else MAX_VOCAB}")
     dev = logits.device
