@@ -102,8 +102,8 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
 
     ``a`` [M, K]: float rows, which the call turns into 8 bits (:func:`quantize_rows`), or :class:`Int8Rows`.  ``w`` [N, K] int8, rows at
     multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.  ``residual`` has the type of the result; ``out`` may be the same tensor, and
-    shares no memory with ``a`` and ``w``.  The result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else
-    bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
+    shares no memory with anything else that is read.  The result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float
+    rows, else bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
     rows = isinstance(a, Int8Rows)
     x = a.q if rows else a
     gated = epilogue == "swiglu"
@@ -145,6 +145,9 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
         place = _place(out)
         if _meet(*place, *_place(x)) or _meet(*place, *_place(w)):
             _refuse("out shares memory with a or w")
+        for v in (w_scale, bias, a.scale if rows else None):
+            if v is not None and _over(place, v):
+                _refuse("out shares memory with factors or the bias")
         if residual is not None and _meet(*place, *_place(residual)) and (out.data_ptr() != residual.data_ptr() or out.stride() != residual.stride()):
             _refuse("out is the residual itself or shares no memory with it")
     if not x.is_cuda:
@@ -203,6 +206,11 @@ def _meet(a, rows_a, pitch_a, width_a, b, rows_b, pitch_b, width_b) -> bool:
         beside = (b - a) % pitch_a
         return beside < width_a or beside + width_b > pitch_a
     return True
+
+
+def _over(place, v):
+    """Whether a matrix (:func:`_place`) shares memory with a contiguous vector, which may lie beside its rows."""
+    return _meet(*place, v.data_ptr(), 1, place[2], v.numel() * v.element_size())
 
 
 def _place(t):
