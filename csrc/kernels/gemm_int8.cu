@@ -1,7 +1,7 @@
 // Products in 8-bit integers:  y[t, n] = s[t] c[n] sum_k q[t, k] w[n, k]  (+ bias)(+ residual) | silu(gate) up.
 //
 // q are rows of activations in 8 bits with a factor s each (int8_rows.cuh), w a weight with a factor c per channel.  The sums are whole
-// numbers in 32 bits, exact for K up to 131072 (128 * 127 * K < 2^31), so their order does not matter and a product may be cut along K
+// numbers in 32 bits, exact for K up to 131072 (q is -127 to 127, w may be -128: 127 * 128 * K < 2^31), so their order does not matter and a product may be cut along K
 // wherever it pays; one rounding to the type of the result follows the factors, the bias and the residual.
 //
 // What bounds it: few rows, the stream of w from HBM (half of bf16's); many, the tensor cores, kind::i8 at twice the rate of

@@ -17,7 +17,7 @@ import torch
 from . import _native, _raw_stream, _timed, current_index, launch_counts, reference, status_ptr
 
 ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-MAX_K = 131072          # sums of 128 * 127 * K stay below 2^31
+MAX_K = 131072          # sums of 127 * 128 * K stay below 2^31: codes of rows are -127 to 127, weights may be -128
 MAX_ROWS = 1 << 30       # of rows and of channels
 MAX_HIDDEN = 16384      # a row of block_norm stays in registers
 _EPI = ("none", "residual", "swiglu")
@@ -27,7 +27,8 @@ _pack_norm = struct.Struct("23q3dq").pack
 
 
 class Int8Rows(NamedTuple):
-    """Rows in 8 bits: ``q`` [rows, k] int8 whose rows begin at multiples of 16 bytes, ``scale`` [rows] fp32; a row stands for ``q * scale``."""
+    """Rows in 8 bits: ``q`` [rows, k] int8, -127 to 127, whose rows begin at multiples of 16 bytes, ``scale`` [rows] fp32; a row stands for
+    ``q * scale``."""
     q: torch.Tensor
     scale: torch.Tensor
 
@@ -100,10 +101,10 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     """``out[M, N] = a @ (w * w_scale[:, None])^T (+ bias) (+ residual)``, or SwiGLU over a :func:`quantize_gate_up` weight (``epilogue="swiglu"``,
     out [M, N / 2]).
 
-    ``a`` [M, K]: float rows, which the call turns into 8 bits (:func:`quantize_rows`), or :class:`Int8Rows`.  ``w`` [N, K] int8, rows at
-    multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.  ``residual`` has the type of the result; ``out`` may be the same tensor, and
-    shares no memory with anything else that is read.  The result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float
-    rows, else bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
+    ``a`` [M, K]: float rows, which the call turns into 8 bits (:func:`quantize_rows`), or :class:`Int8Rows` (codes of -127 to 127: at the largest
+    K a sum of -128 times -128 would pass 32 bits).  ``w`` [N, K] int8, rows at multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.
+    ``residual`` has the type of the result; ``out`` may be the same tensor, and shares no memory with anything else that is read.  The
+    result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
     rows = isinstance(a, Int8Rows)
     x = a.q if rows else a
     gated = epilogue == "swiglu"
