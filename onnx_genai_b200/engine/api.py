@@ -56,7 +56,9 @@ class GenerateOptions:
     stop: tuple = ()                 # stop strings
     stop_token_ids: tuple = ()
     ignore_eos: bool = False
-    logprobs: int = 0                # top-N log-probabilities per generated token (0 = off)
+    # top-N log-probabilities per generated token (0 = off).  Greedy requests on one GPU get them on the device, from sums in 32 bits (off by about 1e-6
+    # and by 2^-22 of the largest logit: less than the logits' own rounding to bf16); others on the host, from sums in 64
+    logprobs: int = 0
     priority: int = 0
     tenant: int = 0
     speculative: bool = False
