@@ -839,16 +839,19 @@ __global__ void __launch_bounds__(kAttnThreads) paged_prefill_fp8_kernel(const _
   };
   if (b_begin < b_end) request_scale(b_begin);
   for (int b = b_begin; b < b_end; ++b) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase))) { ok = false; break; }
-    const uint8_t* raw = stages + stage * kRawStage;
-    // warp w expands page w of the block (K and V) into the shared bf16 tiles
-    expand_page(raw + warp * kRawPage, tile_k + warp * kWorkPage, lane, 32, p.kv_fmt);
-    expand_page(raw + (4 + warp) * kRawPage, tile_v + warp * kWorkPage, lane, 32, p.kv_fmt);
-    if (lane < 2) sc_sh[warp * 2 + lane] = sc_next;
-    if (b + 1 < b_end) request_scale(b + 1);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty_bar[stage]);   // the raw bytes are no longer needed
-    compute_bar_sync();
+    const bool there = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase));
+    if (there) {
+      const uint8_t* raw = stages + stage * kRawStage;
+      // warp w expands page w of the block (K and V) into the shared bf16 tiles
+      expand_page(raw + warp * kRawPage, tile_k + warp * kWorkPage, lane, 32, p.kv_fmt);
+      expand_page(raw + (4 + warp) * kRawPage, tile_v + warp * kWorkPage, lane, 32, p.kv_fmt);
+      if (lane < 2) sc_sh[warp * 2 + lane] = sc_next;
+      if (b + 1 < b_end) request_scale(b + 1);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[stage]);   // the raw bytes are no longer needed
+    }
+    // each warp's wait has a clock of its own: where one ran out, all four leave together
+    if (!compute_bar_all(there)) { ok = false; break; }
     float s[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f; }

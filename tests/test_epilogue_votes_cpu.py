@@ -35,3 +35,22 @@ def test_the_epilogues_vote_before_any_warp_leaves_a_tile(path, name, vote):
     line = body[body.rindex("\n", 0, wait):body.index("\n", wait)]
     assert vote in line, "each warp goes by its own wait:" + line
     assert "continue;" not in body[:wait]
+
+
+def _loop(path, first):
+    """The text of the loop whose body begins with `first` (a regular expression), from there to its closing brace."""
+    with open(os.path.join(KERNELS, path), encoding="utf-8") as f:
+        text = f.read()
+    start = re.search(first, text).start()
+    depth = 0
+    for i in range(start, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth < 0:
+            return text[start:i]
+    raise AssertionError(path)
+
+
+def test_prefill_over_expanded_pages_leaves_its_loop_as_one():
+    body = _loop("attention_fp8.cu", r"[^\n]*mbar_wait\(&full_bar\[stage\], phase\)[^\n]*\n(?=[^}]*// warp w expands page w)")
+    assert body.count("break;") == 1 and re.search(r"if \(!compute_bar_all\(there\)\) \{ ok = false; break; \}", body)
+    assert body.index("compute_bar_all(there)") < body.index("compute_bar_sync()")
