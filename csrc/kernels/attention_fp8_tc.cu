@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(kTcThreads) paged_decode_e4m3_tc_kernel(const 
 #pragma unroll
     for (int g = 0; g < 8; ++g) { m_ref[g] = -INFINITY; l_run[g] = 0.f; }
     bool ok = true;
+    int owed = 1;               // barriers that a warp whose wait ran out still has to meet the others in: one a block and the last
     for (int i = 0; i < n_blocks; ++i) {
       const int s = i % kTcStages, b = i & 1;
       stamp.begin();
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads) paged_decode_e4m3_tc_kernel(const 
       stamp.lap(3);
       ok = ok && tc_wait(&sh.v_full[s], (i / kTcStages) & 1, abort_flag);
       stamp.lap(4);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; owed = n_blocks - i + 1; break; }
       tc_fence_after();
       uint32_t c[16];
       tmem_ld_32x16(lane_base + 16 * b, c);
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads) paged_decode_e4m3_tc_kernel(const 
         }
         if (i > 0) {                                        // O^T holds blocks 0 .. i - 1 once PV(i - 1) has retired
           ok = tc_wait(&sh.p_free[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; owed = n_blocks - i; break; }
           tc_fence_after();
           uint32_t o[16];
           tmem_ld_32x16(lane_base + 32, o);
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads) paged_decode_e4m3_tc_kernel(const 
       }
       if (i >= 2) {                                         // the P buffer is free once PV(i - 2) has retired
         ok = tc_wait(&sh.p_free[b], ((i >> 1) - 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; owed = n_blocks - i; break; }
       }
       stamp.lap(8);
       uint8_t* pt = p_tile + b * kTcSmallTile + (t & 15);
@@ -452,6 +453,7 @@ __global__ void __launch_bounds__(kTcThreads) paged_decode_e4m3_tc_kernel(const 
     if (ok) ok = __all_sync(0xffffffffu, tc_wait(&sh.o_done, 0, abort_flag));
     if (!ok) {
       if (lane == 0) { sh.abort_flag = 1; atomicOr(p.status, kStatusWaitTimeout); }
+      for (; owed > 0; --owed) compute_bar_sync();          // the others' waits may have ended in time
     } else {
       tc_fence_after();
       uint32_t o[16];

@@ -6,13 +6,15 @@ group, between barriers of that group; after its last tile it meets all warps of
 there while another's still sees them.  What has to hold: whatever the waits do, every warp reaches the end of the kernel.
 
 ``vote=False`` lets each warp go by its own wait: the checker finds a warp that skips the tile and others that stay in the group's barrier.
+``owes=True`` lets it, too, but sends the warp through all barriers that it has not been in yet (csrc/kernels/attention_fp8_tc.cu, one a block of keys and
+one behind them), which costs nothing where no wait runs out.
 """
 from __future__ import annotations
 
 from ..utils.model_check import Result, explore
 
 
-def check(warps: int = 4, tiles: int = 2, barriers: int = 2, vote: bool = True) -> Result:
+def check(warps: int = 4, tiles: int = 2, barriers: int = 2, vote: bool = True, owes: bool = False) -> Result:
     # A warp: (tile, place, ok, went).  place 0: waits; 1: meets the group for the vote; 2 .. barriers + 1: the group's barriers; "end": the block's.
     # complete: how many tiles' sums are there.
     init = (((0, 0, True, False),) * warps, 0)
@@ -34,7 +36,9 @@ def check(warps: int = 4, tiles: int = 2, barriers: int = 2, vote: bool = True) 
                 ends.append(("gives up", False))
             for what, seen in ends:
                 # one that gave up before waits no longer and, with a vote, does not ask for another
-                if not ok or not (vote or seen):
+                if owes:
+                    nxt = (tile, 2, ok and seen, seen)
+                elif not ok or not (vote or seen):
                     nxt = after(tile, False)
                 elif vote:
                     nxt = (tile, 1, ok, seen)

@@ -54,3 +54,20 @@ def test_prefill_over_expanded_pages_leaves_its_loop_as_one():
     body = _loop("attention_fp8.cu", r"[^\n]*mbar_wait\(&full_bar\[stage\], phase\)[^\n]*\n(?=[^}]*// warp w expands page w)")
     assert body.count("break;") == 1 and re.search(r"if \(!compute_bar_all\(there\)\) \{ ok = false; break; \}", body)
     assert body.index("compute_bar_all(there)") < body.index("compute_bar_sync()")
+
+
+def test_a_warp_that_meets_the_barriers_it_owes_leaves_nobody_behind():
+    r = epilogue_votes.check(3, 3, 1, vote=False, owes=True)
+    assert r.ok and r.states > 10, str(r)
+
+
+def test_decode_over_one_byte_pages_counts_the_barriers_that_a_warp_owes():
+    body = _loop("attention_fp8_tc.cu", r"      const int s = i % kTcStages, b = i & 1;\n      stamp.begin\(\);\n      ok = ")
+    with open(os.path.join(KERNELS, "attention_fp8_tc.cu"), encoding="utf-8") as f:
+        behind = f.read().split(body)[1]
+    # one barrier a block, and one behind the loop for warps that got that far
+    assert body.count("compute_bar_sync();") == 1 and behind[:behind.index("__syncthreads()")].count("compute_bar_sync();") == 2
+    ahead, rest = body.split("compute_bar_sync();")
+    assert ahead.count("break;") == ahead.count("owed = n_blocks - i + 1; break;") == 1
+    assert rest.count("break;") == rest.count("owed = n_blocks - i; break;") == 2
+    assert "for (; owed > 0; --owed) compute_bar_sync();" in behind[:behind.index("} else {")]
