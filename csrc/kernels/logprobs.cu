@@ -229,7 +229,7 @@ OGB_DEVICE void lp_load(const T* x, int i0, int vocab, uint32_t (&w)[8]) {
 template <typename T, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, TOP ? 4 : 5) logprobs_kernel(const LogprobsParams p) {
   using Type = LpType<T>;
-  constexpr int kPer = Type::kPer, kUnroll = 1;                   // 32-byte pieces a round
+  constexpr int kPer = Type::kPer;                              // values of a 32-byte piece
   __shared__ LpShared<T> sh;
   extern __shared__ __align__(16) uint8_t dynamic_smem[];
   typename Type::Max* piece_max = reinterpret_cast<typename Type::Max*>(dynamic_smem);
@@ -253,58 +253,48 @@ __global__ void __launch_bounds__(kLpThreads, TOP ? 4 : 5) logprobs_kernel(const
   Float2 s2(0.f), t2(0.f);
   int rank = 0;
   const Float2 log2e(1.4426950408889634f);
-  // the next pieces are on their way while these are summed
-  uint32_t next[kUnroll][8];
-  auto fetch = [&](int b) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (b + u * kLpThreads < n_pieces) lp_load(x, first + (b + u * kLpThreads) * kPer, p.vocab, next[u]);
+  // the next piece is on its way while this one is summed
+  uint32_t next[8];
+  auto fetch = [&](int piece) {
+    if (piece < n_pieces) lp_load(x, first + piece * kPer, p.vocab, next);
   };
   fetch(tid);
-  for (int b = tid; b < n_pieces; b += kLpThreads * kUnroll) {
-    uint32_t w[kUnroll][8];
+  for (int piece = tid; piece < n_pieces; piece += kLpThreads) {
+    uint32_t w[8];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[u][j] = next[u][j];
-    fetch(b + kLpThreads * kUnroll);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int piece = b + u * kLpThreads;
-      if (piece < n_pieces) {
-        const float top = Type::max_of(w[u]);
-        if (top - ref > kLpSlack || (ref == -INFINITY && top > -INFINITY)) {
-          if (ref != -INFINITY) {
-            const float d = fmaxf(ref - top, -1000.f);      // a type's lowest value is minus infinity apart, in effect
-            const Float2 r(__expf(d));
-            t2 = r * fma2(Float2(d), s2, t2);
-            s2 = r * s2;
-          }
-          ref = top;
-          neg = -top;
-        }
-        const Float2 minus(neg);
-        Type::pairs(w[u], [&](Float2 v) {
-          const Float2 d = v + minus, a = d * log2e;
-          const Float2 e(ex2_approx(a.lo()), ex2_approx(a.hi()));
-          s2 = s2 + e;
-          if (ENTROPY) t2 = fma2(e, Float2(fmaxf(d.lo(), -1000.f), fmaxf(d.hi(), -1000.f)), t2);
-        });
-        if (top > given) rank += Type::above(w[u], given);
-        if (TOP) {
-          float kept = top;
-          const int i0 = first + piece * kPer;
-          if (is_edge(i0)) {                                // without what is not there
-            kept = __uint_as_float(0x7fc00000u);
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-              if (i0 + j >= 0 && i0 + j < p.vocab) kept = fmaxf(kept, Type::value(w[u], j));
-          }
-          if constexpr (Type::kElem == kElemF32) piece_max[piece] = kept;
-          else if constexpr (Type::kElem == kElemBf16) piece_max[piece] = __float2bfloat16(kept);
-          else piece_max[piece] = __float2half_rn(kept);
-        }
+    for (int j = 0; j < 8; ++j) w[j] = next[j];
+    fetch(piece + kLpThreads);
+    const float top = Type::max_of(w);
+    if (top - ref > kLpSlack || (ref == -INFINITY && top > -INFINITY)) {
+      if (ref != -INFINITY) {
+        const float d = fmaxf(ref - top, -1000.f);          // a type's lowest value is minus infinity apart, in effect
+        const Float2 r(__expf(d));
+        t2 = r * fma2(Float2(d), s2, t2);
+        s2 = r * s2;
       }
+      ref = top;
+      neg = -top;
+    }
+    const Float2 minus(neg);
+    Type::pairs(w, [&](Float2 v) {
+      const Float2 d = v + minus, a = d * log2e;
+      const Float2 e(ex2_approx(a.lo()), ex2_approx(a.hi()));
+      s2 = s2 + e;
+      if (ENTROPY) t2 = fma2(e, Float2(fmaxf(d.lo(), -1000.f), fmaxf(d.hi(), -1000.f)), t2);
+    });
+    if (top > given) rank += Type::above(w, given);
+    if (TOP) {
+      float kept = top;
+      const int i0 = first + piece * kPer;
+      if (is_edge(i0)) {                                    // without what is not there
+        kept = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (i0 + j >= 0 && i0 + j < p.vocab) kept = fmaxf(kept, Type::value(w, j));
+      }
+      if constexpr (Type::kElem == kElemF32) piece_max[piece] = kept;
+      else if constexpr (Type::kElem == kElemBf16) piece_max[piece] = __float2bfloat16(kept);
+      else piece_max[piece] = __float2half_rn(kept);
     }
   }
   LpState st{ref, s2.lo() + s2.hi(), t2.lo() + t2.hi()};
