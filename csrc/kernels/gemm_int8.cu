@@ -1,8 +1,8 @@
 // Products in 8-bit integers:  y[t, n] = s[t] c[n] sum_k q[t, k] w[n, k]  (+ bias)(+ residual) | silu(gate) up.
 //
 // q are rows of activations in 8 bits with a factor s each (int8_rows.cuh), w a weight with a factor c per channel.  The sums are whole
-// numbers in 32 bits, exact for K up to 131072 (q is -127 to 127, w may be -128: 127 * 128 * K < 2^31), so their order does not matter and a product may be cut along K
-// wherever it pays; one rounding to the type of the result follows the factors, the bias and the residual.
+// numbers in 32 bits, exact for K up to 131072 (q is -127 to 127, w may be -128: 127 * 128 * K < 2^31), so their order does not matter and a
+// product may be cut along K wherever it pays; one rounding to the type of the result follows the factors, the bias and the residual.
 //
 // What bounds it: few rows, the stream of w from HBM (half of bf16's); many, the tensor cores, kind::i8 at twice the rate of
 // kind::f16 for the same bytes of operands.
@@ -22,8 +22,9 @@
 //     whole tiles;
 //   * one or two rows of a weight of moderate size: no tensor cores (gemv_int8_kernel).
 //
-// Measured with weights from HBM, 8-bit rows made by the call: 64 rows against 3584 x 18944 with a residual 22 us; 77, gated 37888 x 3584 31;
-// 8192, 3584 x 18944 rows 93 and product 347, 3.2 POP/s; one row of 4608 x 3584 7.4.
+// Measured with weights from HBM, 8-bit rows made by the call: 64 rows against 3584 x 18944 with a residual 22.6 us (28 tiles in clusters of four: as many of
+// five do not fit the SMs' groups at once, and 36 SMs idle); 77, gated 37888 x 3584 32; 8192, 3584 x 18944 rows 97 and product 329 to 349, 3.2 to 3.4
+// POP/s, by the clock that the power limit leaves; one row of 4608 x 3584 9.5.
 #include <algorithm>
 #include <type_traits>
 
@@ -958,9 +959,12 @@ struct Int8Plan {
   bool clusters, pair;
   long long counter_bytes, ws_bytes;
 };
-// The rows of a tile come from an estimate in us: a k-block of a full tile (128 x 256) 0.43 on 148 SMs, of which 0.1 are W's; an epilogue 1 and, over
-// 256 rows, 2 more; a cluster's sum 1.5.  Whole rounds waste what the last leaves idle; ranges cost about 80 k-blocks (partial sums written, awaited
-// and added).  What that chooses, and what as few tiles as possible take:
+// The rows of a tile come from a score that ranks its heights and is no forecast of times: a k-block of a full tile (128 x 256) counts 0.43, of which 0.1
+// are W's; an epilogue 1 and, over 256 rows, 2 more; a cluster's sum 1.5.  It leaves out the stream of W from HBM and counts an epilogue that
+// nothing hides too low (5.8 us a tile of 128 x 256, measured at K = 128): 64 rows against 3584 x 18944 score 8.5 and take 19 to 23 us, 1333 against
+// 1001 x 2039 4.9 and 12.3, 8192 against 3584 x 18944 423 and 329 to 349.  What stands below is what chose the numbers.  Whole rounds
+// waste what the last leaves idle; ranges cost about 80 k-blocks (partial sums written, awaited and added).  What that chooses, and what as few tiles as
+// possible take:
 //   700 rows against 4608 x 3584: four tiles of 176 rows 17.8 us, three of 240 20.4;  1333, 1001 x 2039: 17 of 80 rows 11.6, six of 224 14.1
 //   1000, gated 9728 x 896: eleven of 96 rows 25.6, eight of 128 30.4
 //   ranges: 1500, 3584 x 18944 123 -> 93, 8192 419 -> 401; but 2000, 3584 x 3584 49 -> 62, 4096, 8192 x 8192 193 -> 203
