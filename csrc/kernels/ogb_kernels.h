@@ -269,7 +269,8 @@ int ogb_sample_f32(const float* logits, int* out_tokens, const float* temperatur
 // quantize_rows: factor = max |x| / 127, q = round(127 x / max |x|) of every row.
 int ogb_quantize_rows(const void* x, void* q, float* factor, int rows, int cols, int64_t ldx, int64_t ldq, int elem, void* stream);
 // out = (q w^T) factor channel (+ bias)(+ residual), or silu(gate) up of it over blocks of 128 gate and 128 up rows of w (gated, N of them together).
-// Either x, float rows that the call quantises, or q (codes of -127 to 127: sums of K up to 131072 then fit 32 bits) and factor; ws: ogb_gemm_int8_workspace bytes for this call alone, 256-byte aligned.
+// Either x, float rows that the call quantises, or q (codes of -127 to 127: sums of K up to 131072 then fit 32 bits) and factor; ws:
+// ogb_gemm_int8_workspace bytes for this call alone, 256-byte aligned.
 int64_t ogb_gemm_int8_workspace(int M, int N, int K, int gated, int quantize);
 int ogb_gemm_int8(const void* x, int x_elem, int64_t ldx, const void* q, const float* factor, int64_t ldq, const void* w, int64_t ldw,
                   const float* channel, const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldc, int out_elem, int M, int N,

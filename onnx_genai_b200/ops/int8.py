@@ -104,7 +104,8 @@ def gemm_int8(a, w, w_scale, bias=None, residual=None, epilogue="none", out=None
     ``a`` [M, K]: float rows, which the call turns into 8 bits (:func:`quantize_rows`), or :class:`Int8Rows` (codes of -127 to 127: at the largest
     K a sum of -128 times -128 would pass 32 bits).  ``w`` [N, K] int8, rows at multiples of 16 bytes; ``w_scale`` and ``bias`` [N] fp32.
     ``residual`` has the type of the result; ``out`` may be the same tensor, and shares no memory with anything else that is read.  The
-    result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else bf16.  Sums over K are exact; one rounding follows the factors, the bias and the residual."""
+    result's type is ``out_dtype``, that of ``out`` or of ``residual``, or that of float rows, else bf16.  Sums over K are exact; one rounding
+    follows the factors, the bias and the residual."""
     rows = isinstance(a, Int8Rows)
     x = a.q if rows else a
     gated = epilogue == "swiglu"

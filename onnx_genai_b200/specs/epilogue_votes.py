@@ -5,7 +5,7 @@ For every tile a warp waits until the tile's sums are complete, at most for a ti
 group, between barriers of that group; after its last tile it meets all warps of the block.  The wait of one warp may run out just before the sums are
 there while another's still sees them.  What has to hold: whatever the waits do, every warp reaches the end of the kernel.
 
-``vote=False`` lets each warp go by its own wait: the checker finds a warp that skips the tile and others that stay in the group's barrier.
+``vote=False`` lets each warp go by its own wait: the search finds a warp that skips the tile and others that stay in the group's barrier.
 ``owes=True`` lets it, too, but sends the warp through all barriers that it has not been in yet (csrc/kernels/attention_fp8_tc.cu, one a block of keys and
 one behind them), which costs nothing where no wait runs out.
 """
